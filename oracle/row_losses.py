@@ -1,0 +1,79 @@
+"""The losses on rows of scores in numpy, straight from their definitions, in extended precision so that a Float64 kernel's error
+is not compared with the same rounding here (test infrastructure only).
+
+Each returns the value, the gradient and the sizes that rounding acts on, from which the tests derive their tolerances."""
+import numpy as np
+
+L = np.longdouble
+
+
+def _log_softmax(z):
+    with np.errstate(invalid="ignore", divide="ignore"):
+        m = z.max()
+        return z - m - np.log(np.exp(z - m).sum())
+
+
+def distillation(x, t, idx, *, temperature=1.0, lam=1.0, teacher_lse=None, weights=None, labels=None, label_lam=0.0):
+    """(f, gradient, size of the gradient's terms, size of the value's terms): rows of x one by one"""
+    x = np.asarray(x, L)
+    n, v = x.shape
+    f, f_size = L(0), L(0)
+    grad, size = np.zeros((n, v), L), np.zeros((n, v), L)
+    log2e = L(1) / np.log(L(2))
+    temperature, lam, label_lam = L(temperature), L(lam), L(label_lam)
+    for i in range(n):
+        w = L(1) if weights is None else L(weights[i])
+        if w == 0:
+            continue
+        bad = np.isnan(x[i]).any() or (len(idx[i]) and (np.min(idx[i]) < -1 or np.max(idx[i]) >= v))
+        y = -1 if labels is None else int(labels[i])
+        if bad or y < -1 or y >= v:
+            f = np.nan
+            grad[i] = np.nan
+            continue
+        if np.all(x[i] == -np.inf):
+            continue
+        on = np.asarray(idx[i]) >= 0
+        cls = np.asarray(idx[i])[on]
+        tt = np.asarray(t[i], L)[on] / temperature
+        lq = _log_softmax(x[i] / temperature)
+        q = np.exp(lq)
+        far = np.where(q > 0, (x[i][np.isfinite(x[i])].max() - x[i]) * log2e, 0.0)  # how far an entry's exponent is from the largest's
+        if teacher_lse is not None:
+            lp = tt - L(teacher_lse[i])
+        else:
+            lp = _log_softmax(tt) if len(tt) and tt.max() > -np.inf else np.full(len(tt), -np.inf)
+        p = np.exp(lp)
+        phat, ksize = np.zeros(v, L), np.zeros(v, L)
+        np.add.at(phat, cls, p)
+        with np.errstate(invalid="ignore"):
+            np.add.at(ksize, cls, np.where(p > 0, p * (64 + 4 * np.abs(lp)), 0.0))
+        pr, rest = L(0), np.zeros(v, L)
+        outside = np.ones(v, bool)
+        outside[cls] = False
+        if teacher_lse is not None and len(tt) and outside.any():
+            pr = max(L(0), L(1) - p.sum())
+            qr = q[outside].sum()
+            rest[outside] = pr / qr if qr > 0 else 0.0
+        elif teacher_lse is not None and len(tt) == 0:
+            pr, qr, rest = L(1), L(1), np.ones(v, L)  # nothing listed: the outside class is everything on both sides
+        mass = p.sum() + pr
+        with np.errstate(invalid="ignore", divide="ignore"):
+            terms = np.where(p > 0, p * (lp - lq[cls]), 0.0)
+            sizes = np.where(p > 0, p * (64 + 8 * (np.abs(lp) + np.abs(lq[cls]) + np.abs(x[i][cls]) / temperature)), 0.0)
+            row = terms.sum() + (pr * (np.log(pr) - np.log(qr)) if pr > 0 else 0.0)
+            row_size = sizes[np.isfinite(sizes)].sum() + (64 * pr * (1 + abs(np.log(pr)) + abs(np.log(qr))) + 64 * (1 + abs(np.log(qr))) if pr > 0 and qr > 0 else 0.0)
+        f += lam * w * row
+        f_size += lam * w * row_size
+        grad[i] = lam * w / temperature * (mass * q - phat - rest * q)
+        size[i] = lam * w / temperature * ((mass + rest) * q * (64 + 6 * far / temperature) + ksize)
+        if y >= 0:
+            ls = _log_softmax(x[i])
+            one = np.zeros(v, L)
+            one[y] = 1
+            f -= label_lam * w * ls[y]
+            if np.isfinite(ls[y]):
+                f_size += label_lam * w * (64 + 8 * (abs(ls[y]) + 2 * abs(x[i][y])))
+            grad[i] += label_lam * w * (np.exp(ls) - one)
+            size[i] += label_lam * w * (np.exp(ls) * (64 + 6 * far) + one)
+    return float(f), grad.astype(np.float64), size.astype(np.float64), float(f_size)

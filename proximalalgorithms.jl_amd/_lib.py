@@ -8,6 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("PG_LIB_PATH") or os.path.join(HERE, "libproxgrad_hip.so")
 
 PG_F32, PG_F64 = 0, 1
+PG_BF16, PG_F16 = 2, 3  # include/proxgrad_hip_rows.h: scores and gradients of the row losses
 PG_G_ZERO, PG_G_NORML1, PG_G_INDBOX, PG_G_SQRNORML2 = 0, 1, 2, 3
 PG_SEQ_ADAPTIVE, PG_SEQ_FIXED, PG_SEQ_SIMPLE, PG_SEQ_CONSTANT, PG_SEQ_HOST, PG_SEQ_REPEATED = 0, 1, 2, 3, 4, 5
 PG_FLAG_GAMMA_TOO_SMALL, PG_FLAG_SWEEP_FALLBACK, PG_FLAG_COOP_SLOW = 1, 2, 4
@@ -167,6 +168,21 @@ SIGNATURES = {
     "pg_lbfgs_images_apply": [_vp, _vp, _vp],
     "pg_lbfgs_images_ready": [_vp, C.POINTER(_i32)],
 }
+
+class pg_distill(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("classes", C.c_int64), ("top", C.c_int64), ("teacher", C.c_void_p), ("teacher_ld", C.c_int64),
+                ("index", C.c_void_p), ("index_ld", C.c_int64), ("teacher_lse", C.c_void_p), ("weights", C.c_void_p),
+                ("labels", C.c_void_p), ("teacher_dtype", C.c_int32), ("index_bits", C.c_int32), ("lse_dtype", C.c_int32),
+                ("weights_dtype", C.c_int32), ("label_bits", C.c_int32), ("reserved", C.c_int32), ("temperature", C.c_double),
+                ("lam", C.c_double), ("label_lam", C.c_double)]
+
+
+# include/proxgrad_hip_rows.h (versioned by itself; the boundary's table above stays what proxgrad_hip.h / _ext.h declare)
+PG_ROWS_ABI_VERSION = 1
+ROW_SIGNATURES = {
+    "pg_distill_value_and_gradient": [_vp, C.POINTER(pg_distill), _i32, _vp, _i64, _vp, _i64, _vp, _pf64],
+}
+
 _SPECIAL = {"pg_abi_version": ([], C.c_int32), "pg_last_error": ([], C.c_char_p), "pg_comm_available": ([], C.c_int32)}
 
 _lib = None
@@ -198,6 +214,18 @@ def load():
         fn = getattr(lib, name)  # AttributeError if the symbol is not exported
         fn.argtypes = argtypes
         fn.restype = C.c_int32
+    try:
+        lib.pg_rows_abi_version.argtypes, lib.pg_rows_abi_version.restype = [], C.c_int32
+        found = int(lib.pg_rows_abi_version())
+    except AttributeError:
+        found = None
+    if found != PG_ROWS_ABI_VERSION:
+        raise ProxGradError(f"{LIB_PATH} has version {found} of the row losses, this package was written against {PG_ROWS_ABI_VERSION}: "
+                            "rebuild it (`python proximalalgorithms.jl_amd/_build.py --force`)")
+    for name, argtypes in ROW_SIGNATURES.items():
+        fn = getattr(lib, name)
+        fn.argtypes = argtypes
+        fn.restype = C.c_int32
     for name, (argtypes, restype) in _SPECIAL.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes
@@ -208,6 +236,11 @@ def load():
 
 def exported_symbols():
     return list(SIGNATURES) + list(_SPECIAL)
+
+
+def exported_row_symbols():
+    """the exports include/proxgrad_hip_rows.h declares"""
+    return list(ROW_SIGNATURES) + ["pg_rows_abi_version"]
 
 
 def check(status):

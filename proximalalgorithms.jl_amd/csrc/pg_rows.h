@@ -1,0 +1,171 @@
+// Pieces shared by the losses on rows of scores (pg_rows_distill.hip, pg_rows_balance.hip): element types, 16-byte vectors of
+// them, reductions over a wave and over a workgroup.
+#pragma once
+#include "pg_internal.h"
+#include "proxgrad_hip_rows.h"
+
+namespace pgrows {
+
+// ---- host ----
+inline bool dtype_ok(int dt) { return dt == PG_F32 || dt == PG_F64 || dt == PG_BF16 || dt == PG_F16; }
+inline int dtype_size(int dt) { return dt == PG_F64 ? 8 : (dt == PG_F32 ? 4 : 2); }
+
+// A context's device for the length of a call (the caller's current device may be another one)
+struct DeviceScope {
+  int prev = -1;
+  bool changed = false;
+  pg_status st = PG_OK;
+  explicit DeviceScope(int device) {
+    if (hipGetDevice(&prev) != hipSuccess) prev = -1;
+    if (prev != device) {
+      if (hipSetDevice(device) != hipSuccess) {
+        pg_set_error("hipSetDevice(%d) failed", device);
+        st = PG_ERR_HIP;
+      } else {
+        changed = true;
+      }
+    }
+  }
+  ~DeviceScope() {
+    if (changed && prev >= 0) (void)hipSetDevice(prev);
+  }
+};
+
+// The context's workspaces are ordered by its stream; a graph that somebody else records from that stream could be replayed next to it
+inline pg_status refuse_foreign_capture(pg_ctx* c) {
+  if (c->capturing) return PG_OK;
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  const hipError_t e = hipStreamIsCapturing(c->stream, &cs);
+  if (e != hipSuccess) (void)hipGetLastError();
+  if (e != hipSuccess || cs != hipStreamCaptureStatusNone) {
+    pg_set_error("the context's stream is being captured by somebody else: record with pg_ctx_capture_begin / pg_ctx_capture_end");
+    return PG_ERR_UNSUPPORTED;
+  }
+  return PG_OK;
+}
+
+#ifdef __HIPCC__
+// ---- device ----
+template <typename T, int N>
+using vec = T __attribute__((ext_vector_type(N)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Elem;  // compute type, elements per 16 bytes
+template <>
+struct Elem<float> {
+  using C = float;
+  static constexpr int N = 4;
+};
+template <>
+struct Elem<double> {
+  using C = double;
+  static constexpr int N = 2;
+};
+template <>
+struct Elem<__bf16> {
+  using C = float;
+  static constexpr int N = 8;
+};
+template <>
+struct Elem<_Float16> {
+  using C = float;
+  static constexpr int N = 8;
+};
+
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::C up(T v) {
+  return (typename Elem<T>::C)v;
+}
+// 16 bytes at an address that is a multiple of the element's size only: one dwordx4 access on gfx950 (unaligned access mode)
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+  u32x4 v;
+};
+template <typename T>
+__device__ __forceinline__ u32x4 ld16(const T* p) {
+  return reinterpret_cast<const Loose<T>*>(p)->v;
+}
+template <typename T>
+__device__ __forceinline__ void st16(T* p, u32x4 v) {
+  reinterpret_cast<Loose<T>*>(p)->v = v;
+}
+template <typename T>
+__device__ __forceinline__ void unpack(u32x4 u, typename Elem<T>::C (&f)[Elem<T>::N]) {
+  using VT = vec<T, Elem<T>::N>;
+  const VT e = __builtin_bit_cast(VT, u);
+#pragma unroll
+  for (int i = 0; i < Elem<T>::N; ++i) f[i] = (typename Elem<T>::C)e[i];
+}
+template <typename T>
+__device__ __forceinline__ u32x4 pack(const typename Elem<T>::C (&f)[Elem<T>::N]) {
+  vec<T, Elem<T>::N> e;
+#pragma unroll
+  for (int i = 0; i < Elem<T>::N; ++i) e[i] = (T)f[i];  // the one rounding of a gradient entry
+  return __builtin_bit_cast(u32x4, e);
+}
+
+__device__ __forceinline__ double ld_real(const void* p, int dt, int64_t i) {
+  switch (dt) {
+    case PG_F64: return ((const double*)p)[i];
+    case PG_F32: return (double)((const float*)p)[i];
+    case PG_BF16: return (double)(float)((const __bf16*)p)[i];
+    default: return (double)(float)((const _Float16*)p)[i];
+  }
+}
+__device__ __forceinline__ int64_t ld_int(const void* p, int bits, int64_t i) {
+  return bits == 64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
+}
+
+__device__ __forceinline__ float ex2(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ double ex2(double v) { return exp2(v); }
+__device__ __forceinline__ float lg2(float v) { return __builtin_amdgcn_logf(v); }
+__device__ __forceinline__ double lg2(double v) { return log2(v); }
+template <typename C>
+struct Lim;
+template <>
+struct Lim<float> {
+  static constexpr float lowest = -3.402823466e+38f;
+};
+template <>
+struct Lim<double> {
+  static constexpr double lowest = -1.7976931348623157e+308;
+};
+
+template <typename C>
+__device__ __forceinline__ C wave_sum(C v) {
+  return pg_wave_allreduce<false, C>(v);
+}
+__device__ __forceinline__ float fmx(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double fmx(double a, double b) { return fmax(a, b); }
+// maximum over the 16 lanes of a DPP row / over the wave, NaN passed over (the sums carry it)
+template <typename C>
+__device__ __forceinline__ C row16_max(C v) {
+  v = fmx(v, pg_dpp_mov<0xB1>(v));
+  v = fmx(v, pg_dpp_mov<0x4E>(v));
+  v = fmx(v, pg_dpp_mov<0x141>(v));
+  return fmx(v, pg_dpp_mov<0x140>(v));
+}
+template <typename C>
+__device__ __forceinline__ C wave_max(C v) {
+  v = row16_max(v);
+  return fmx(fmx(pg_readlane(v, 0), pg_readlane(v, 16)), fmx(pg_readlane(v, 32), pg_readlane(v, 48)));
+}
+template <typename C>
+__device__ __forceinline__ C row16_sum(C v) {
+  return pg_row_allreduce<false, C>(v);
+}
+
+// NT threads of one workgroup work on a row: all of it (a workgroup's barrier) or one wave of it (its LDS accesses are in order)
+template <int NT>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (NT == 64) {
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
+}
+#endif  // __HIPCC__
+
+}  // namespace pgrows

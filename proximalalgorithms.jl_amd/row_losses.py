@@ -1,0 +1,246 @@
+"""Smooth losses whose scores come in rows, one softmax per row: terms for classifiers, re-rankers and routers.
+
+They stand beside ``LogisticLoss`` and ``SquaredDistance`` (one score per sample) and honour the same surface,
+``value_and_gradient(u, out=None) -> (f(u), grad)``, so ``Composed(loss, A)``, ``SlicedSeparableSum`` and every iteration of the
+package take them: ``u`` is then a :class:`HIPVector` holding the rows one after another.  They also take the scores as a 2-D torch
+tensor on the device (Float32, Float64, bfloat16 or Float16; rows any distance apart), as a training program has them, and
+``value_and_gradient_async`` leaves the value on the device, so that nothing waits.
+
+A loss runs on its context's stream.  Called under another current torch stream, it waits for that stream's work and that
+stream waits for the loss.  One host thread per context at a time; a graph is recorded with ``Context.capture_begin`` (with ``out``
+and ``value`` given: nothing can be allocated while recording)."""
+import ctypes as C
+
+import numpy as np
+
+from . import _lib
+from ._lib import PG_BF16, PG_F16, PG_F32, PG_F64, ProxGradError, call
+from .device import HIPVector, get_context
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+_DTYPES = {}
+
+
+def _dtype_code(dt):
+    if not _DTYPES:
+        torch = _torch()
+        _DTYPES.update({torch.float32: PG_F32, torch.float64: PG_F64, torch.bfloat16: PG_BF16, torch.float16: PG_F16})
+    return _DTYPES.get(dt)
+
+
+def _as_tensor(x, name):
+    """x as a torch tensor, wherever it lives"""
+    torch = _torch()
+    if isinstance(x, HIPVector):
+        return x.torch()
+    if isinstance(x, torch.Tensor):
+        return x
+    return torch.from_numpy(np.ascontiguousarray(x))
+
+
+def _rows_of(x, name, shape, kinds, convert):
+    """x checked against ``shape`` and brought to one of ``kinds`` (else to ``convert``), last axis dense"""
+    t = _as_tensor(x, name)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype not in kinds:
+        if t.is_floating_point() != convert.is_floating_point or t.is_complex():
+            raise TypeError(f"{name} has element type {t.dtype}")
+        t = t.to(convert)
+    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    return t
+
+
+def _common_device(tensors, ctx):
+    """the context: given, or that of the device the tensors live on"""
+    devices = {t.device.index for t in tensors if t is not None and t.is_cuda}
+    if len(devices) > 1:
+        raise ValueError("the loss's tensors live on different devices")
+    if ctx is None:
+        ctx = get_context(devices.pop() if devices else None)
+    elif devices and devices != {ctx.device}:
+        raise ValueError("the loss's tensors live on another device than its context")
+    return ctx
+
+
+class _Ordered:
+    """the call's kernels run on the context's stream: between the current torch stream's past and its future"""
+
+    __slots__ = ("ctx", "cur", "ext")
+
+    def __init__(self, ctx):
+        self.ctx = ctx
+
+    def __enter__(self):
+        torch = _torch()
+        ctx = self.ctx
+        self.cur = None
+        if ctx.capturing:
+            return
+        cur = torch.cuda.current_stream(ctx.torch_device)
+        if cur.cuda_stream != ctx.stream:
+            with torch.cuda.device(ctx.device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise ProxGradError("a torch graph is being recorded: record with Context.capture_begin instead",
+                                        code=_lib.PG_ERR_UNSUPPORTED)
+                self.cur, self.ext = cur, torch.cuda.ExternalStream(ctx.stream, device=ctx.torch_device)
+                self.ext.wait_stream(cur)
+
+    def __exit__(self, *exc):
+        if self.cur is not None:
+            with _torch().cuda.device(self.ctx.device):
+                self.cur.wait_stream(self.ext)
+
+
+class _RowLoss:
+    """Checks of the scores and of ``out``, shared by the row losses; a subclass has ``rows``, ``classes``, ``ctx``, ``_evaluate``."""
+
+    is_generalized_quadratic = False
+
+    def _locate(self, u, name):
+        """(pointer, row distance, dtype code) of scores or gradients"""
+        n, v = self.rows, self.classes
+        if isinstance(u, HIPVector):
+            if u.n != n * v:
+                raise ValueError(f"{name} must hold {n} x {v} scores, got {u.n}")
+            if u.ctx.device != self.ctx.device:
+                raise ValueError(f"{name} lives on another device than the loss")
+            return u.ptr, max(v, 1), u.pg_dtype
+        code = _dtype_code(getattr(u, "dtype", None))
+        if code is None:
+            raise TypeError(f"{name} must be a HIPVector or a Float32, Float64, bfloat16 or Float16 torch tensor")
+        if not u.is_cuda or u.device.index != self.ctx.device:
+            raise ValueError(f"{name} must live on the loss's device {self.ctx.device}")
+        if tuple(u.shape) != (n, v) and not (u.dim() == 1 and u.shape[0] == n * v and (n * v == 0 or u.stride(0) == 1)):
+            raise ValueError(f"{name} must have shape ({n}, {v}), got {tuple(u.shape)}")
+        if u.dim() == 1:
+            return u.data_ptr(), max(v, 1), code
+        if v > 1 and u.stride(1) != 1:
+            raise ValueError(f"the scores of a row of {name} must be adjacent (stride 1)")
+        ld = u.stride(0) if n > 1 else max(v, 1)
+        if ld < v:
+            raise ValueError(f"the rows of {name} overlap")
+        return u.data_ptr(), ld, code
+
+    def _like(self, u):
+        if isinstance(u, HIPVector):
+            return u.similar()
+        if self.ctx.capturing:
+            raise ProxGradError("device allocation during stream capture: give out and value")
+        return _torch().empty(u.shape, dtype=u.dtype, device=u.device)
+
+    def _place(self, u, out):
+        """arguments of the entry point for scores ``u`` and gradient ``out`` (made if None)"""
+        up, uld, code = self._locate(u, "u")
+        if out is None:
+            out = self._like(u)
+        op, old, ocode = self._locate(out, "out")
+        if ocode != code:
+            raise TypeError("out must have the scores' element type")
+        if self.rows and self.classes and not (op == up and (old == uld or self.rows == 1)):
+            size = 8 if code == PG_F64 else (4 if code == PG_F32 else 2)
+            reach = ((self.rows - 1) * uld + self.classes) * size, ((self.rows - 1) * old + self.classes) * size
+            if op < up + reach[0] and up < op + reach[1]:
+                gap = ((op - up) % (uld * size)) if uld == old else 0  # side by side in one buffer is fine
+                if not (uld == old and self.classes * size <= gap <= (uld - self.classes) * size):
+                    raise ValueError("out overlaps u: it may be u itself or apart from it")
+        return out, (up, uld, op, old, code)
+
+    def value_and_gradient(self, u, out=None):
+        """(f(u), grad f(u)); waits for the value.  ``out``: where the gradient goes (may be ``u`` itself)"""
+        out, where = self._place(u, out)
+        f = C.c_double()
+        with _Ordered(self.ctx):
+            self._evaluate(where, None, C.byref(f))
+        return (u.dtype.type(f.value) if isinstance(u, HIPVector) else f.value), out
+
+    def value_and_gradient_async(self, u, out=None, value=None):
+        """The same without waiting: the value is a one-element torch tensor on the device (Float32; Float64 for Float64 scores)"""
+        torch = _torch()
+        out, where = self._place(u, out)
+        vdt = torch.float64 if where[4] == PG_F64 else torch.float32
+        if value is None:
+            if self.ctx.capturing:
+                raise ProxGradError("device allocation during stream capture: give out and value")
+            value = torch.empty((), dtype=vdt, device=self.ctx.torch_device)
+        elif value.numel() != 1 or value.dtype != vdt or not value.is_cuda or value.device.index != self.ctx.device:
+            raise ValueError(f"value must be a one-element {vdt} tensor on the loss's device")
+        with _Ordered(self.ctx):
+            self._evaluate(where, value.data_ptr(), None)
+        return value, out
+
+    def __call__(self, u):
+        scratch = getattr(self, "_scratch", None)
+        if scratch is None or type(scratch) is not type(u) or scratch.dtype != u.dtype:
+            scratch = self._scratch = self._like(u)
+        return self.value_and_gradient(u, out=scratch)[0]
+
+
+class DistillationLoss(_RowLoss):
+    """Distillation from a teacher's top logits (include/proxgrad_hip_rows.h: pg_distill_value_and_gradient).
+
+    ``teacher_logits`` (rows x top) at classes ``teacher_index`` (rows x top; -1: no entry), temperature T, per-row ``weights``:
+
+        f(u) = lam sum_n w_n KL(p_n || softmax(u_n / T)) + label_lam sum_n w_n (log sum exp u_n - u_n[y_n])
+
+    p is the softmax of the listed logits / T; with ``teacher_lse`` -- log sum exp of ALL the teacher's logits / T per row -- it is the
+    teacher's own probability, and the classes outside the list count as one more class (then f is not convex).  ``labels``: -1 = none.
+    The usual factor T^2 is the caller's: ``lam=T**2``.  Rows of weight 0 are not read.  Tensors on the device are used where
+    they are, later changes included; host arrays are checked and uploaded.  An index or label that is out of range on the
+    device makes the value and that row's gradient NaN."""
+
+    def __init__(self, teacher_logits, teacher_index, n_classes, *, temperature=1.0, lam=1.0, teacher_lse=None, weights=None,
+                 labels=None, label_lam=0.0, ctx=None):
+        torch = _torch()
+        t = _as_tensor(teacher_logits, "teacher_logits")
+        if t.dim() != 2:
+            raise ValueError("teacher_logits must be a (rows, top) array")
+        self.rows, top = int(t.shape[0]), int(t.shape[1])
+        self.classes = int(n_classes)
+        if self.classes < 0 or self.classes >= 1 << 30:
+            raise ValueError("n_classes must be between 0 and 2^30 - 1")
+        if top > 1024:
+            raise ValueError("at most 1024 listed logits per row")
+        self.temperature, self.lam, self.label_lam = float(temperature), float(lam), float(label_lam)
+        if not (self.temperature > 0 and np.isfinite(self.temperature)):
+            raise ValueError("temperature must be positive and finite")
+        if not (self.lam >= 0 and self.label_lam >= 0 and np.isfinite(self.lam) and np.isfinite(self.label_lam)):
+            raise ValueError("lam and label_lam must be nonnegative and finite")
+        if labels is None and self.label_lam:
+            raise ValueError("label_lam without labels")
+        reals, ints = (torch.float32, torch.float64), (torch.int32, torch.int64)
+        t = _rows_of(t, "teacher_logits", (self.rows, top), (*reals, torch.bfloat16, torch.float16), torch.float32)
+        index = _rows_of(teacher_index, "teacher_index", (self.rows, top), ints, torch.int64)
+        lse = None if teacher_lse is None else _rows_of(teacher_lse, "teacher_lse", (self.rows,), reals, torch.float32)
+        weights = None if weights is None else _rows_of(weights, "weights", (self.rows,), reals, torch.float32)
+        labels = None if labels is None else _rows_of(labels, "labels", (self.rows,), ints, torch.int64)
+        for name, v in (("teacher_index", index), ("labels", labels)):
+            if v is not None and not v.is_cuda and v.numel() and not (int(v.min()) >= -1 and int(v.max()) < self.classes):
+                raise ValueError(f"{name} must lie between -1 and n_classes - 1")
+        if weights is not None and not weights.is_cuda and weights.numel() and not bool((weights >= 0).all()):
+            raise ValueError("weights must be nonnegative")
+        self.is_convex = lse is None
+        self.ctx = _common_device((t, index, lse, weights, labels), ctx)
+        dev = self.ctx.torch_device
+        self._keep = t, index, lse, weights, labels = [None if v is None else v.to(dev) for v in (t, index, lse, weights, labels)]
+        ptr = lambda v: None if v is None else v.data_ptr()  # noqa: E731
+        bits = lambda v: 64 if v is not None and v.dtype == torch.int64 else 32  # noqa: E731
+        code = lambda v: PG_F32 if v is None else _dtype_code(v.dtype)  # noqa: E731
+        self._d = _lib.pg_distill(rows=self.rows, classes=self.classes, top=top, teacher=ptr(t),
+                                  teacher_ld=t.stride(0) if self.rows > 1 else top, index=ptr(index),
+                                  index_ld=index.stride(0) if self.rows > 1 else top, teacher_lse=ptr(lse), weights=ptr(weights),
+                                  labels=ptr(labels), teacher_dtype=code(t), index_bits=bits(index), lse_dtype=code(lse),
+                                  weights_dtype=code(weights), label_bits=bits(labels), temperature=self.temperature, lam=self.lam,
+                                  label_lam=self.label_lam)
+        self._dref = C.byref(self._d)
+
+    def _evaluate(self, where, value, f_out):
+        up, uld, op, old, code = where
+        call("pg_distill_value_and_gradient", self.ctx.handle, self._dref, code, up, uld, op, old, value, f_out)

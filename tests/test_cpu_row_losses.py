@@ -1,0 +1,94 @@
+"""Row losses without a GPU: the header and its binding agree, every refusal comes before any device work, the oracle's gradients
+are the differences of its values."""
+import ctypes as C
+import os
+import re
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import row_losses as ref
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_header_and_binding_agree(tmp_path):
+    import subprocess
+
+    import __graft_entry__ as ge
+
+    ge.build()
+    from proximalalgorithms.jl_amd import _lib
+
+    text = open(os.path.join(ROOT, "include", "proxgrad_hip_rows.h")).read()
+    declared = set(re.findall(r"^\s*(?:pg_status|int32_t)\s+(pg_[a-z0-9_]+)\s*\(", text, flags=re.M))
+    assert declared == set(_lib.exported_row_symbols())
+    lib = _lib.load()
+    assert all(hasattr(lib, s) for s in declared)
+    assert lib.pg_rows_abi_version() == _lib.PG_ROWS_ABI_VERSION == int(re.search(r"#define PG_ROWS_ABI_VERSION (\d+)", text).group(1))
+    structs = [("pg_distill", _lib.pg_distill)]
+    src = ['#include <stdio.h>', '#include <stddef.h>', '#include "proxgrad_hip_rows.h"', "int main(void) {"]
+    for name, s in structs:
+        src.append(f'printf("%zu\\n", sizeof({name}));')
+        src += [f'printf("%zu\\n", offsetof({name}, {f[0]}));' for f in s._fields_]
+    (tmp_path / "a.c").write_text("\n".join(src + ["return 0; }"]))
+    subprocess.run(["gcc", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(tmp_path / "a.c"), "-o", str(tmp_path / "a")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "a")], capture_output=True, text=True, check=True).stdout.split()]
+    want = []
+    for _, s in structs:
+        want += [C.sizeof(s)] + [getattr(s, f[0]).offset for f in s._fields_]
+    assert got == want
+
+
+def test_distillation_refusals():
+    import proximalalgorithms.jl_amd as pa
+
+    t, i = np.zeros((3, 2), np.float32), np.zeros((3, 2), np.int64)
+    bad = [
+        (ValueError, (t[0], i, 5), {}), (ValueError, (t, i[:2], 5), {}), (ValueError, (t, i + 5, 5), {}), (ValueError, (t, i - 2, 5), {}),
+        (ValueError, (t, i, -1), {}), (ValueError, (t, i, 1 << 30), {}), (TypeError, (t, t, 5), {}), (TypeError, (i, i, 5), {}),
+        (ValueError, (np.zeros((1, 1025), np.float32), np.zeros((1, 1025), int), 2000), {}),
+        (ValueError, (t, i, 5), dict(temperature=0.0)), (ValueError, (t, i, 5), dict(temperature=float("inf"))),
+        (ValueError, (t, i, 5), dict(lam=-1.0)), (ValueError, (t, i, 5), dict(lam=float("nan"))), (ValueError, (t, i, 5), dict(label_lam=1.0)),
+        (ValueError, (t, i, 5), dict(labels=np.array([0, 5, 0]), label_lam=1.0)), (ValueError, (t, i, 5), dict(labels=np.array([0, 1]))),
+        (ValueError, (t, i, 5), dict(weights=np.array([1.0, -1.0, 0.0]))), (ValueError, (t, i, 5), dict(weights=np.ones(4))),
+        (ValueError, (t, i, 5), dict(teacher_lse=np.ones(2))), (TypeError, (t, i, 5), dict(teacher_lse=np.ones(3, int))),
+        (TypeError, (t, i, 5), dict(labels=np.ones(3))),
+    ]
+    for err, args, kw in bad:
+        with pytest.raises(err):
+            pa.DistillationLoss(*args, **kw)
+    if not torch.cuda.is_available():
+        with pytest.raises(pa.ProxGradError):
+            pa.DistillationLoss(t, i, 5)  # valid: and then there is no device, and no fallback
+
+
+def test_c_entry_refuses_before_any_device_work():
+    from proximalalgorithms.jl_amd import _lib
+
+    lib = _lib.load()
+    assert lib.pg_distill_value_and_gradient(None, None, 0, None, 0, None, 0, None, None) == _lib.PG_ERR_INVALID
+    assert b"null" in lib.pg_last_error()
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_oracle_distillation_gradient_is_its_differences(rest):
+    rng = np.random.default_rng(3)
+    n, v, k = 3, 11, 4
+    x = rng.normal(size=(n, v))
+    t, idx = rng.normal(size=(n, k)) + 2, np.stack([rng.permutation(v)[:k] for _ in range(n)])
+    idx[0, 3] = -1
+    idx[1, 2] = idx[1, 0]
+    kw = dict(temperature=1.7, lam=0.8, weights=np.array([1.0, 0.5, 2.0]), labels=np.array([-1, 2, idx[2, 0]]), label_lam=0.4)
+    if rest:
+        kw["teacher_lse"] = np.log(np.exp(t / 1.7).sum(1)) + 0.4
+    g = ref.distillation(x, t, idx, **kw)[1]
+    h = 1e-5
+    for i in range(n):
+        for j in range(v):
+            xp, xm = x.copy(), x.copy()
+            xp[i, j] += h
+            xm[i, j] -= h
+            d = (ref.distillation(xp, t, idx, **kw)[0] - ref.distillation(xm, t, idx, **kw)[0]) / (2 * h)
+            assert abs(d - g[i, j]) < 1e-8  # second-order difference: h^2 times a third derivative of order one, plus eps / h
