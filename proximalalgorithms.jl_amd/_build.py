@@ -9,14 +9,15 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "libproxgrad_hip.so")
-SOURCES = ["pg_core.hip", "pg_gemv.hip", "pg_gemv_tn2.hip", "pg_gemv_tn3.hip", "pg_gemv_tn4.hip", "pg_gemv_tn4d.hip", "pg_gemv_tn5.hip", "pg_gemv_dys.hip", "pg_vec.hip", "pg_iter.hip", "pg_persist.hip", "pg_lbfgs.hip", "pg_comm.hip", "pg_rows_distill.hip"]
+SOURCES = ["pg_core.hip", "pg_gemv.hip", "pg_gemv_tn2.hip", "pg_gemv_tn3.hip", "pg_gemv_tn4.hip", "pg_gemv_tn4d.hip", "pg_gemv_tn5.hip", "pg_gemv_dys.hip", "pg_vec.hip", "pg_iter.hip", "pg_persist.hip", "pg_lbfgs.hip", "pg_comm.hip", "pg_rows_distill.hip", "pg_rows_distill_f32.hip", "pg_rows_distill_f64.hip", "pg_rows_distill_bf16.hip",
+           "pg_rows_distill_f16.hip"]
 # every header under csrc/ and include/ (pg_gemv_tn4.hip is also compiled a second time, as pg_gemv_tn4d.hip's body)
 HEADERS = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")) + [os.path.join(CSRC, "pg_gemv_tn4.hip"), os.path.join(INCLUDE, "proxgrad_hip.h"), os.path.join(INCLUDE, "proxgrad_hip_ext.h"), os.path.join(INCLUDE, "proxgrad_hip_rows.h")]
 # headers that only the row losses (pg_rows_*.hip) see
-ROW_HEADERS = {os.path.join(CSRC, "pg_rows.h"), os.path.join(INCLUDE, "proxgrad_hip_rows.h")}
+ROW_HEADERS = {os.path.join(CSRC, "pg_rows.h"), os.path.join(CSRC, "pg_rows_distill.h"), os.path.join(INCLUDE, "proxgrad_hip_rows.h")}
 ARCH = "gfx950"
 # the row losses are compiled without the packed Float32 instructions (hipcc's host pass warns that it does not know the feature)
-SOURCE_FLAGS = {"pg_rows_distill.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}
+ROW_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():
@@ -46,7 +47,7 @@ def build(force=False, verbose=True):
         objs.append(o)
         deps = HEADERS if src.startswith("pg_rows_") else [h for h in HEADERS if h not in ROW_HEADERS]
         if force or _stale(o, [s] + deps):
-            cmd = [hipcc] + flags + SOURCE_FLAGS.get(src, []) + ["-c", s, "-o", o]
+            cmd = [hipcc] + flags + (ROW_FLAGS if src.startswith("pg_rows_") else []) + ["-c", s, "-o", o]
             if verbose:
                 print(" ".join(cmd), flush=True)
             jobs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))

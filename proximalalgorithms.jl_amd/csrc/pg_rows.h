@@ -90,6 +90,28 @@ template <typename T>
 __device__ __forceinline__ void st16(T* p, u32x4 v) {
   reinterpret_cast<Loose<T>*>(p)->v = v;
 }
+// vector v of a row: a wave-uniform base and a 32-bit offset (a row is at most 2^30 elements of at most 8 bytes: the product is unsigned)
+template <typename T>
+__device__ __forceinline__ T* at16(T* base, int v) {
+  return (T*)((uintptr_t)base + (uint64_t)(unsigned)v * 16u);
+}
+// A row as a buffer resource: base and length in scalar registers, one 32-bit offset per lane; a load behind the end gives 0, a
+// store behind it is dropped (the hardware's bounds check), so no vector needs a mask or a 64-bit address of its own.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);
+}
+__device__ __forceinline__ u32x4 ldb16(__amdgpu_buffer_rsrc_t r, int byte) { return __builtin_amdgcn_raw_buffer_load_b128(r, byte, 0, 0); }
+__device__ __forceinline__ void stb16(__amdgpu_buffer_rsrc_t r, int byte, u32x4 v) { __builtin_amdgcn_raw_buffer_store_b128(v, r, byte, 0, 0); }
+// 16 bytes of -inf
+template <typename T>
+__device__ __forceinline__ u32x4 minus_inf16() {
+  vec<T, Elem<T>::N> e;
+#pragma unroll
+  for (int i = 0; i < Elem<T>::N; ++i) e[i] = (T)-INFINITY;
+  return __builtin_bit_cast(u32x4, e);
+}
+// a value the compiler knows nothing about any more
+__device__ __forceinline__ void opaque(u32x4& v) { asm volatile("" : "+v"(v)); }
 template <typename T>
 __device__ __forceinline__ void unpack(u32x4 u, typename Elem<T>::C (&f)[Elem<T>::N]) {
   using VT = vec<T, Elem<T>::N>;
@@ -117,10 +139,49 @@ __device__ __forceinline__ int64_t ld_int(const void* p, int bits, int64_t i) {
   return bits == 64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
 }
 
+// the same for what is the same in every lane and never written by the kernel that reads it (one value per row): scalar loads
+#define PG_CONST_AS __attribute__((address_space(4)))
+__device__ __forceinline__ double ld_real_u(const void* p, int dt, int64_t i) {  // PG_F32 or PG_F64
+  return dt == PG_F64 ? ((const PG_CONST_AS double*)p)[i] : (double)((const PG_CONST_AS float*)p)[i];
+}
+__device__ __forceinline__ int64_t ld_int_u(const void* p, int bits, int64_t i) {
+  return bits == 64 ? ((const PG_CONST_AS int64_t*)p)[i] : (int64_t)((const PG_CONST_AS int32_t*)p)[i];
+}
+__device__ __forceinline__ float uniform(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))); }
+__device__ __forceinline__ double uniform(double v) { return pg_readlane(v, 0); }
+
 __device__ __forceinline__ float ex2(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ double ex2(double v) { return exp2(v); }
 __device__ __forceinline__ float lg2(float v) { return __builtin_amdgcn_logf(v); }
 __device__ __forceinline__ double lg2(double v) { return log2(v); }
+// exp(x) in Float64 from its series: x = n ln 2 + r, |r| <= ln(2) / 2, sum of r^k / k! up to k = 12 (the next term is below 2^-52
+// of the sum), times 2^n.  The library's exp inside a loop keeps its constants in some forty vector registers around the
+// loop, which a kernel that holds a row in registers has not got; here they pass through scalar registers where they are used.
+__device__ __forceinline__ double scalar_const(double v) {
+  asm volatile("" : "+s"(v));
+  return v;
+}
+__device__ __forceinline__ double exp_series(double x) {
+  const double n = rint(x * 1.4426950408889634);
+  double r = fma(n, scalar_const(-0x1.62e42fefa38p-1), x);  // ln 2 in two pieces, the first with zeros at its end
+  r = fma(n, scalar_const(-0x1.ef35793c7673p-45), r);
+  double p = scalar_const(1.0 / 479001600.0);
+  p = fma(p, r, scalar_const(1.0 / 39916800.0));
+  p = fma(p, r, scalar_const(1.0 / 3628800.0));
+  p = fma(p, r, scalar_const(1.0 / 362880.0));
+  p = fma(p, r, scalar_const(1.0 / 40320.0));
+  p = fma(p, r, scalar_const(1.0 / 5040.0));
+  p = fma(p, r, scalar_const(1.0 / 720.0));
+  p = fma(p, r, scalar_const(1.0 / 120.0));
+  p = fma(p, r, scalar_const(1.0 / 24.0));
+  p = fma(p, r, scalar_const(1.0 / 6.0));
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  p = ldexp(p, (int)fmax(fmin(n, 2000.0), -2000.0));
+  return x < -745.2 ? 0.0 : (x > 709.8 ? (double)INFINITY : p);  // (NaN stays NaN)
+}
+
 template <typename C>
 struct Lim;
 template <>

@@ -1,0 +1,796 @@
+// Kernels of the distillation loss (pg_rows_distill.hip has the entry point; one translation unit per element type).
+//
+// Per row, with z = x / T, e_v = exp(z_v - max z), S = sum e, q = e / S, the listed classes and their p:
+//   L = sum_k p_k (log p_k - log q_k) + p_r (log p_r - log Q_r),     Q_r = sum of q outside the list
+//   dL/dx_v = ((sum p + p_r) q_v - phat_v - [v not listed] p_r q_v / Q_r) / T
+// so outside the list the gradient is ONE multiple of e_v, and only the listed classes (and the label) need more: every
+// vector is written with the unlisted coefficient, then a few threads overwrite the listed entries.  Q_r is summed over
+// the unlisted classes themselves (1 - sum of the listed q loses everything where the student agrees with the teacher),
+// which a bitmap of the row in LDS makes possible; the bitmap also finds classes listed twice.
+#pragma once
+#include <algorithm>
+
+#include "pg_rows.h"
+
+
+namespace pgrows {
+
+struct DArgs;
+pg_status distill_f32(pg_ctx* c, const DArgs& a, int64_t rows);
+pg_status distill_f64(pg_ctx* c, const DArgs& a, int64_t rows);
+pg_status distill_bf16(pg_ctx* c, const DArgs& a, int64_t rows);
+pg_status distill_f16(pg_ctx* c, const DArgs& a, int64_t rows);
+
+constexpr double LOG2E = 1.4426950408889634;
+constexpr double LN2 = 0.6931471805599453;
+constexpr int BIT0 = 8;         // bits in front of a chunk's first aligned vector (the head of a misaligned row: at most 7)
+constexpr int STAT = 6;         // doubles per (row, part)
+constexpr int MAX_PARTS = 64;   // one lane each when a row's parts are joined
+constexpr int MAX_TOP = 1024;
+
+struct DArgs {
+  const void* x;
+  void* g;
+  const void *t, *idx, *lse, *w, *lab;
+  int64_t ldx, ldg, ldt, ldi, row0, nrows;  // rows of this launch
+  int V, K, tdt, ibits, lsedt, wdt, labbits;
+  double invT, lam, lab_lam;
+  int parts, pv;  // parts of a row, 16-byte vectors per part
+  double *stat, *xk;
+  double *partials, *acc, *out;
+  unsigned* counter;
+  void* value;
+  int first, last;  // of the launches of this call
+};
+
+namespace {
+
+// ---- one row's scalars, from the statistics over the whole row ----------------------------------------------------
+template <typename C>
+struct RowScal {
+  C M, cB, cR, c1;  // reference score; coefficients of e at listed / unlisted classes, of exp(x - M) for labels at T != 1
+  C ql, qy;         // what a unit of teacher mass / the label takes off
+  C ls, ls1;        // log sum exp((x - M) / T) and log sum exp(x - M)
+  double pr, log_qr;
+  bool empty;
+};
+template <typename C>
+__device__ __forceinline__ RowScal<C> row_scalars(const DArgs& a, bool tail, bool two, double w, bool has_label, C M, C s_rest, C s_list, C s1,
+                                                  C n_listed, double mass) {
+  RowScal<C> r;
+  const C S = tail ? s_rest + s_list : s_rest;
+  r.empty = S == C(0);  // every score -inf (the largest score always contributes 1)
+  r.M = M;
+  r.ls = lg2(S) * (C)LN2;
+  r.ql = (C)(a.lam * w * a.invT);
+  r.qy = has_label ? (C)(a.lab_lam * w) : C(0);
+  C rest = C(0);
+  r.pr = 0.0;
+  r.log_qr = 0.0;
+  if (tail) {
+    if ((int64_t)n_listed < a.V) {  // the list may hold every class: then nothing is outside it
+      const double left = 1.0 - mass;
+      r.pr = left > 0.0 ? left : (left == left ? 0.0 : left);
+      const C qr = s_rest / S;
+      r.log_qr = (double)(lg2(qr) * (C)LN2);
+      rest = (r.pr > 0.0 && qr > C(0)) ? (C)r.pr / qr : C(0);
+    }
+  }
+  const C total = (C)(mass + r.pr);
+  r.cB = r.ql * total / S;
+  r.cR = tail ? r.ql * (total - rest) / S : r.cB;
+  r.c1 = C(0);
+  r.ls1 = r.ls;
+  if (two) {
+    r.c1 = r.qy / s1;
+    r.ls1 = lg2(s1) * (C)LN2;
+  } else {  // labels at T = 1 share e
+    r.cB += r.qy / S;
+    r.cR += r.qy / S;
+  }
+  if (r.empty) {
+    r.cB = r.cR = r.c1 = r.ql = r.qy = C(0);
+    r.M = Lim<C>::lowest;
+  }
+  return r;
+}
+
+// probability of a listed entry: log p and p
+template <typename C>
+__device__ __forceinline__ void entry_p(const DArgs& a, int64_t row, int k, double norm, C& lp, C& p) {
+  const double t = ld_real(a.t, a.tdt, row * a.ldt + k) * a.invT;
+  lp = (C)(t == -INFINITY ? t : t - norm);  // (a list of -inf only has norm -inf)
+  p = ex2(lp * (C)LOG2E);
+}
+
+// ---- a row's place in memory: head elements up to the first 16-byte boundary, whole vectors, tail -----------------
+template <typename T>
+struct Place {
+  int h, nmain, hV;
+  __device__ __forceinline__ Place(const T* xr, int V) {
+    constexpr int N = Elem<T>::N;
+    const int off = (int)((reinterpret_cast<uintptr_t>(xr) & 15u) / sizeof(T));
+    h = off ? N - off : 0;
+    h = h < V ? h : V;
+    nmain = (V - h) / N;
+    hV = h + nmain * N;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ unsigned listed_bits(const unsigned* bm, int vbit) {  // of the vector whose first bit is vbit (a multiple of N)
+  constexpr int N = Elem<T>::N;
+  return (bm[vbit >> 5] >> (vbit & 31)) & ((1u << N) - 1u);
+}
+
+// running maximum and sums of one thread
+template <typename C, bool TAIL, bool TWO>
+struct Run {
+  C m = Lim<C>::lowest, s = C(0), sl = C(0), s1 = C(0), n = C(0);
+  C c;  // log2(e) / T
+  __device__ __forceinline__ void raise(C to) {
+    const C d = m - to;
+    const C f = ex2(d * c);
+    s *= f;
+    if constexpr (TAIL) sl *= f;
+    if constexpr (TWO) s1 *= ex2(d * (C)LOG2E);
+    m = to;
+  }
+  __device__ __forceinline__ void listed(C x) {  // a listed class (TAIL only)
+    if (x > m) raise(x);
+    sl += ex2((x - m) * c);
+    n += C(1);
+  }
+  template <int N>
+  __device__ __forceinline__ void add(const C (&f)[N], unsigned bits) {
+    C vm = f[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) vm = fmx(vm, f[i]);
+    if (vm > m) raise(vm);
+    C e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = ex2((f[i] - m) * c);
+    if constexpr (TAIL) {
+      if (bits) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = (bits >> i) & 1u ? C(0) : e[i];
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < N; o *= 2)
+#pragma unroll
+      for (int i = 0; i < N; i += 2 * o) e[i] += e[i + o];
+    s += e[0];
+    if constexpr (TWO) {
+      C t = C(0);
+#pragma unroll
+      for (int i = 0; i < N; ++i) t += ex2((f[i] - m) * (C)LOG2E);
+      s1 += t;
+    }
+  }
+  __device__ __forceinline__ void add1(C x, bool in_list) {
+    if (x > m) raise(x);
+    if (!(TAIL && in_list)) s += ex2((x - m) * c);
+    if constexpr (TWO) s1 += ex2((x - m) * (C)LOG2E);
+  }
+};
+
+// ---- the general form: a row in parts, two reads ------------------------------------------------------------------
+// Any length, any number of rows.  First launch: the statistics of each part (and the listed scores, which an in-place
+// gradient overwrites); second launch: every part joins its row's statistics and writes its piece of the gradient.
+constexpr int PT = 256;
+
+template <typename T, bool TAIL, bool TWO>
+__global__ __launch_bounds__(PT) void distill_part_stats(DArgs a) {
+  using C = typename Elem<T>::C;
+  constexpr int N = Elem<T>::N;
+  extern __shared__ unsigned bm[];
+  __shared__ C sm[PT / 64][5];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int part = blockIdx.x % a.parts;
+  const int64_t r = blockIdx.x / a.parts, row = a.row0 + r;
+  if (a.w != nullptr && ld_real(a.w, a.wdt, row) == 0.0) return;
+  const T* xr = (const T*)a.x + row * a.ldx;
+  const Place<T> pl(xr, a.V);
+  const int v0 = min(part * a.pv, pl.nmain), v1 = min(v0 + a.pv, pl.nmain);
+  const bool lastp = part == a.parts - 1;
+  const int e0 = part == 0 ? 0 : pl.h + v0 * N, e1 = lastp ? a.V : pl.h + v1 * N;
+  const int bbase = pl.h + v0 * N - BIT0;  // element of bit 0
+  const int words = (a.pv * N + BIT0 + N + 31) / 32;
+  if constexpr (TAIL) {
+    for (int i = tid; i < words; i += PT) bm[i] = 0;
+    __syncthreads();
+  }
+  Run<C, TAIL, TWO> run;
+  run.c = (C)(a.invT * LOG2E);
+  bool bad = false;
+  for (int k = tid; k < a.K; k += PT) {
+    const int64_t id = ld_int(a.idx, a.ibits, row * a.ldi + k);
+    bad |= id < -1 || id >= a.V;
+    if (id >= e0 && id < e1) {
+      const C x = up<T>(xr[id]);
+      a.xk[r * (a.K + 1) + k] = (double)x;
+      if constexpr (TAIL) {
+        const int b = (int)id - bbase;
+        const unsigned old = atomicOr(&bm[b >> 5], 1u << (b & 31));
+        if (!((old >> (b & 31)) & 1u)) run.listed(x);
+      }
+    }
+  }
+  if (tid == 0 && a.lab != nullptr) {
+    const int64_t y = ld_int(a.lab, a.labbits, row);
+    bad |= y < -1 || y >= a.V;
+    if (y >= e0 && y < e1) a.xk[r * (a.K + 1) + a.K] = (double)up<T>(xr[y]);
+  }
+  if constexpr (TAIL) __syncthreads();
+  const T* xm = xr + pl.h;
+  for (int v = v0 + tid; v < v1; v += PT) {
+    C f[N];
+    unpack<T>(ld16(at16(xm, v)), f);
+    run.template add<N>(f, TAIL ? listed_bits<T>(bm, (v - v0) * N + BIT0) : 0u);
+  }
+  // (thread i: the i-th element of the head; thread PT - 1 - i: of the tail)
+  const int ee = part == 0 && tid < pl.h ? tid : (lastp && pl.hV + (PT - 1 - tid) < a.V ? pl.hV + (PT - 1 - tid) : -1);
+  if (ee >= 0) {
+    const int b = ee - bbase;
+    run.add1(up<T>(xr[ee]), TAIL && ((bm[b >> 5] >> (b & 31)) & 1u));
+  }
+  if (bad) run.s = (C)NAN;
+  const C M = wave_max(run.m);
+  const C f = ex2((run.m - M) * run.c);
+  const C s = wave_sum(run.s * f), sl = TAIL ? wave_sum(run.sl * f) : C(0), n = TAIL ? wave_sum(run.n) : C(0);
+  const C s1 = TWO ? wave_sum(run.s1 * ex2((run.m - M) * (C)LOG2E)) : C(0);
+  if (lane == 0) sm[wave][0] = M, sm[wave][1] = s, sm[wave][2] = sl, sm[wave][3] = s1, sm[wave][4] = n;
+  __syncthreads();
+  if (tid == 0) {
+    C m = sm[0][0];
+    for (int i = 1; i < PT / 64; ++i) m = fmx(m, sm[i][0]);
+    C o[4] = {};
+    for (int i = 0; i < PT / 64; ++i) {
+      const C g = ex2((sm[i][0] - m) * run.c);
+      o[0] += sm[i][1] * g;
+      o[1] += sm[i][2] * g;
+      if constexpr (TWO) o[2] += sm[i][3] * ex2((sm[i][0] - m) * (C)LOG2E);
+      o[3] += sm[i][4];
+    }
+    double* st = a.stat + (r * a.parts + part) * STAT;
+    st[0] = (double)m;
+    for (int i = 0; i < 4; ++i) st[1 + i] = (double)o[i];
+  }
+}
+
+template <typename T, bool TAIL, bool TWO>
+__global__ __launch_bounds__(PT) void distill_part_grad(DArgs a) {
+  using C = typename Elem<T>::C;
+  constexpr int N = Elem<T>::N;
+  extern __shared__ unsigned bm[];
+  __shared__ double smd[PT / 64][2];
+  __shared__ int dup;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int part = blockIdx.x % a.parts;
+  const int64_t r = blockIdx.x / a.parts, row = a.row0 + r;
+  const T* xr = (const T*)a.x + row * a.ldx;
+  T* gr = (T*)a.g + row * a.ldg;
+  const Place<T> pl(xr, a.V);
+  const int v0 = min(part * a.pv, pl.nmain), v1 = min(v0 + a.pv, pl.nmain);
+  const bool lastp = part == a.parts - 1;
+  const int e0 = part == 0 ? 0 : pl.h + v0 * N, e1 = lastp ? a.V : pl.h + v1 * N;
+  const int bbase = pl.h + v0 * N - BIT0;
+  const int ee = part == 0 && tid < pl.h ? tid : (lastp && pl.hV + (PT - 1 - tid) < a.V ? pl.hV + (PT - 1 - tid) : -1);
+  const double w = a.w != nullptr ? ld_real(a.w, a.wdt, row) : 1.0;
+  double v_row = 0.0;
+  if (w == 0.0) {
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    for (int v = v0 + tid; v < v1; v += PT) st16(at16(gr + pl.h, v), zero);
+    if (ee >= 0) gr[ee] = (T)0.f;
+  } else {
+    const int words = (a.pv * N + BIT0 + N + 31) / 32;
+    for (int i = tid; i < words; i += PT) bm[i] = 0;
+    if (tid == 0) dup = 0;
+    __syncthreads();
+    const int64_t y = a.lab != nullptr ? ld_int(a.lab, a.labbits, row) : -1;
+    // the teacher's side: log normaliser and listed mass
+    double tm = -INFINITY, ts = 0.0;
+    for (int k = tid; k < a.K; k += PT) {
+      const int64_t id = ld_int(a.idx, a.ibits, row * a.ldi + k);
+      if (id < 0 || id >= a.V) continue;
+      if (id >= e0 && id < e1) {
+        const int b = (int)id - bbase;
+        if ((atomicOr(&bm[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1u) dup = 1;
+      }
+      const double t = ld_real(a.t, a.tdt, row * a.ldt + k) * a.invT;
+      if constexpr (TAIL) {
+        ts += exp(t - ld_real(a.lse, a.lsedt, row));
+      } else if (t > tm || t != t) {
+        ts = t != t ? t : ts * exp(tm - t) + 1.0;
+        if (t > tm) tm = t;
+      } else if (t > -INFINITY) {
+        ts += exp(t - tm);
+      }
+    }
+    const double wm = wave_max(tm);
+    const double wsum = wave_sum(TAIL || tm == -INFINITY ? ts : ts * exp(tm - wm));
+    if (lane == 0) smd[wave][0] = wm, smd[wave][1] = wsum;
+    __syncthreads();
+    tm = smd[0][0];
+    for (int i = 1; i < PT / 64; ++i) tm = fmax(tm, smd[i][0]);
+    ts = 0.0;
+    for (int i = 0; i < PT / 64; ++i) ts += TAIL || smd[i][0] == -INFINITY ? smd[i][1] : smd[i][1] * exp(smd[i][0] - tm);
+    const double norm = TAIL ? ld_real(a.lse, a.lsedt, row) : tm + log(ts);
+    const double mass = TAIL ? ts : (ts == 0.0 ? 0.0 : ts / ts);  // a list without mass: no teacher
+    // the row's parts joined, one lane each
+    const double* st = a.stat + r * a.parts * STAT;
+    const bool in = lane < a.parts;
+    const C pm = in ? (C)st[lane * STAT] : Lim<C>::lowest;
+    const C M = wave_max(pm);
+    const C c = (C)(a.invT * LOG2E);
+    const C f = ex2((pm - M) * c);
+    const C s = wave_sum(in ? (C)st[lane * STAT + 1] * f : C(0));
+    const C sl = TAIL ? wave_sum(in ? (C)st[lane * STAT + 2] * f : C(0)) : C(0);
+    const C s1 = TWO ? wave_sum(in ? (C)st[lane * STAT + 3] * ex2((pm - M) * (C)LOG2E) : C(0)) : C(0);
+    const C nl = TAIL ? wave_sum(in ? (C)st[lane * STAT + 4] : C(0)) : C(0);
+    const RowScal<C> rs = row_scalars<C>(a, TAIL, TWO, w, y >= 0, M, s, sl, s1, nl, mass);
+    for (int v = v0 + tid; v < v1; v += PT) {
+      C x[N], o[N];
+      unpack<T>(ld16(at16(xr + pl.h, v)), x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        o[i] = ex2((x[i] - rs.M) * c) * rs.cR;
+        if constexpr (TWO) o[i] += ex2((x[i] - rs.M) * (C)LOG2E) * rs.c1;
+      }
+      st16(at16(gr + pl.h, v), pack<T>(o));
+    }
+    auto entry = [&](C x, C coef) { return ex2((x - rs.M) * c) * coef + (TWO ? ex2((x - rs.M) * (C)LOG2E) * rs.c1 : C(0)); };
+    if (ee >= 0) gr[ee] = (T)entry(up<T>(xr[ee]), rs.cR);
+    __syncthreads();  // the vectors are written: the listed entries go over them
+    const double* xk = a.xk + r * (a.K + 1);
+    for (int k = tid; k < a.K; k += PT) {
+      const int64_t id = ld_int(a.idx, a.ibits, row * a.ldi + k);
+      if (id < 0 || id >= a.V) continue;
+      C lp, p;
+      entry_p<C>(a, row, k, norm, lp, p);
+      const C x = (C)xk[k];
+      if (part == 0 && !rs.empty && p != C(0)) v_row += a.lam * w * (double)(p * (lp - ((x - rs.M) * (C)a.invT - rs.ls)));
+      if (id >= e0 && id < e1) {
+        C ph = p;
+        bool owner = true;
+        if (dup) {  // a class listed twice: its first entry writes the sum
+          for (int q = 0; q < a.K; ++q) {
+            if (q == k || ld_int(a.idx, a.ibits, row * a.ldi + q) != id) continue;
+            owner &= q > k;
+            C lq, pq;
+            entry_p<C>(a, row, q, norm, lq, pq);
+            ph += pq;
+          }
+        }
+        if (owner) gr[id] = (T)(entry(x, rs.cB) - rs.ql * ph - (id == y ? rs.qy : C(0)));
+      }
+    }
+    if (tid == PT - 1) {
+      if (y >= e0 && y < e1) {
+        const int b = (int)y - bbase;
+        if (!((bm[b >> 5] >> (b & 31)) & 1u)) gr[y] = (T)(entry((C)xk[a.K], rs.cR) - rs.qy);
+      }
+      if (part == 0 && !rs.empty) {
+        if (TAIL && rs.pr != 0.0) v_row += a.lam * w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - rs.log_qr);
+        if (y >= 0 && y < a.V) v_row += a.lab_lam * w * (double)(rs.ls1 - ((C)xk[a.K] - rs.M));
+        if (rs.ls != rs.ls) v_row = NAN;  // a NaN score, or an index or label out of range
+      }
+    }
+  }
+  double v[1] = {v_row}, one[1] = {1.0}, fin[1];
+  if (grid_reduce_finalize<1, 0, PT / 64>(v, a.partials, a.counter, a.acc + 1, one, fin) && threadIdx.x == 0) {
+    const double total = a.first ? fin[0] : *a.acc + fin[0];
+    *a.acc = total;
+    if (a.last) {
+      *a.out = total;
+      if (a.value != nullptr) *(C*)a.value = (C)total;
+    }
+  }
+}
+
+template <typename T, bool TAIL, bool TWO>
+pg_status run_parts(pg_ctx* c, DArgs a, int64_t rows) {
+  constexpr int N = Elem<T>::N;
+  const int64_t vecs = (a.V + N - 1) / N;
+  // a part: at least 1024 vectors (16 KiB), at most what the bitmap holds; enough parts for two workgroups per CU
+  const int64_t most = (32 * 1024 * 8) / N;
+  int64_t parts = (2 * c->num_cu + rows - 1) / rows;
+  parts = std::min<int64_t>(parts, (vecs + 1023) / 1024);
+  parts = std::max<int64_t>(parts, (vecs + most - 1) / most);
+  parts = std::max<int64_t>(1, std::min<int64_t>(parts, MAX_PARTS));
+  a.parts = (int)parts;
+  a.pv = (int)((vecs + parts - 1) / parts);
+  const size_t lds = ((size_t)a.pv * N + BIT0 + N + 31) / 32 * 4 + 4;
+  if (lds > 64 * 1024) {
+    pg_set_error("pg_distill: rows of more than %lld classes are not supported for this type", (long long)(64 * 1024 * 8 / N * N) * MAX_PARTS);
+    return PG_ERR_UNSUPPORTED;
+  }
+  const int64_t ws = (int64_t)PG_RED_MAX_BLOCKS * (PG_RED_MAX_NS - 1) - 8;  // doubles behind the reduction's own partials
+  int64_t batch = std::min<int64_t>(ws / (parts * STAT + a.K + 1), PG_RED_MAX_BLOCKS / parts);
+  a.acc = c->red_partials + PG_RED_MAX_BLOCKS;
+  a.stat = a.acc + 8;
+  for (int64_t r0 = 0; r0 < rows; r0 += batch) {
+    const int64_t nb = std::min<int64_t>(batch, rows - r0);
+    a.row0 = r0;
+    a.nrows = nb;
+    a.xk = a.stat + nb * parts * STAT;
+    a.first = r0 == 0;
+    a.last = r0 + nb == rows;
+    distill_part_stats<T, TAIL, TWO><<<(unsigned)(nb * parts), PT, lds, c->stream>>>(a);
+    PG_LAUNCH_CHECK();
+    distill_part_grad<T, TAIL, TWO><<<(unsigned)(nb * parts), PT, lds, c->stream>>>(a);
+    PG_LAUNCH_CHECK();
+  }
+  return PG_OK;
+}
+
+
+// ---- the row in registers: one read, one write ---------------------------------------------------------------------
+// NT threads hold a row as NV 16-byte vectors each (NT = 64: a wave per row, four rows per workgroup; else a workgroup per row).
+// Pass 1 takes running maximum and sums as the vectors arrive, one reduction joins them, pass 2 writes the gradient from the
+// registers and, as a vector leaves, loads the same vector of the group's NEXT row in its place, so that the memory pipes
+// stay busy through the reduction.  Loads return in order: what the next row's list needs (classes, logits, listed scores)
+// is therefore asked for before its vectors.
+template <typename C>
+struct Ent {  // of one row, per thread: entry tid of the list, the label, the teacher's normaliser, the weight
+  int id, y;  // -1 absent, -2 out of range
+  double lse, w;
+  C t, x, xy;
+};
+
+template <typename T, int NT, int NV>
+struct RowsGeom {
+  using C = typename Elem<T>::C;
+  static constexpr int N = Elem<T>::N;
+  static constexpr int WG = NT < 256 ? 256 : NT;
+  static constexpr int GPW = WG / NT, NW = NT / 64;
+  static constexpr int capacity = NT * NV * N;  // classes a group's registers hold
+  static __host__ __device__ int words(int V) { return ((V + BIT0 + N + 31) / 32 + 1) & ~1; }
+  static __host__ __device__ int group_bytes(int V, int K) {  // bitmap, then two sets (this row's, the next's) of the list's scores, probabilities, classes
+    return words(V) * 4 + (2 * K * (2 * (int)sizeof(C) + 4) + 7) / 8 * 8;
+  }
+};
+
+template <typename T, int NT, int NV, bool tail, bool two>
+__global__ __launch_bounds__((NT < 256 ? 256 : NT)) void distill_rows(DArgs a) {
+  using G = RowsGeom<T, NT, NV>;
+  using C = typename G::C;
+  constexpr int N = G::N, NW = G::NW, GPW = G::GPW;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  __shared__ C sm[GPW][NW][7];
+  __shared__ double smt[GPW][NW];
+  __shared__ int flags[GPW][2][2];  // [row parity][a class is listed twice, the label is listed]
+  const int tid = threadIdx.x % NT, lane = threadIdx.x & 63;
+  const int wave_in_wg = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int grp = NT == 64 ? wave_in_wg : 0, wave = NT == 64 ? 0 : wave_in_wg;
+  const int nwords = G::words(a.V);
+  unsigned* bm = (unsigned*)(lds + G::group_bytes(a.V, a.K) * grp);
+  C* lx = (C*)(bm + nwords);     // [2][K]
+  C* lp = lx + 2 * a.K;          // [2][K]
+  int* li = (int*)(lp + 2 * a.K);  // [2][K]
+#pragma clang loop unroll(disable)
+  for (int i = tid; i < nwords; i += NT) bm[i] = 0;
+  if (tid < 4) flags[grp][tid >> 1][tid & 1] = 0;
+  group_sync<NT>();
+
+  const int64_t stride = (int64_t)gridDim.x * GPW;
+  const C c = (C)(a.invT * LOG2E);
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+
+  // the next row that has a weight (the others' gradients are zeros)
+  auto advance = [&](int64_t row, double& w) {
+    w = 1.0;
+    for (; row < a.nrows; row += stride) {
+      if (a.w == nullptr || (w = ld_real_u(a.w, a.wdt, row)) != 0.0) break;
+      T* gr = (T*)a.g + row * a.ldg;
+      const Place<T> pl(gr, a.V);
+#pragma clang loop unroll(disable)
+      for (int v = tid; v < pl.nmain; v += NT) st16(at16(gr + pl.h, v), zero);
+      if (tid < pl.h) gr[tid] = (T)0.f;
+      if (pl.hV + tid < a.V) gr[pl.hV + tid] = (T)0.f;
+    }
+    return row;
+  };
+  auto ask_list = [&](int64_t row, Ent<C>& e) {
+    e.id = -1, e.y = -1, e.t = (C)-INFINITY, e.lse = 0.0;
+    if (row >= a.nrows) return;
+    if (tid < a.K) {
+      const int64_t id = ld_int(a.idx, a.ibits, row * a.ldi + tid);
+      e.id = id < -1 || id >= a.V ? -2 : (int)id;
+      e.t = (C)ld_real(a.t, a.tdt, row * a.ldt + tid);
+    }
+    if (tail) e.lse = ld_real_u(a.lse, a.lsedt, row);
+    if (a.lab != nullptr) {
+      const int64_t y = ld_int_u(a.lab, a.labbits, row);
+      e.y = y < -1 || y >= a.V ? -2 : (int)y;
+    }
+  };
+  auto ask_listed_scores = [&](int64_t row, Ent<C>& e) {
+    e.x = e.xy = Lim<C>::lowest;
+    if (row >= a.nrows) return;
+    const T* xr = (const T*)a.x + row * a.ldx;
+    if (e.id >= 0) e.x = up<T>(xr[e.id]);
+    if (e.y >= 0) e.xy = up<T>(xr[e.y]);
+  };
+  // head elements: threads 0 ..; tail elements: threads NT - 1 .. down
+  auto edge_of = [&](const Place<T>& pl) { return tid < pl.h ? tid : (pl.hV + (NT - 1 - tid) < a.V ? pl.hV + (NT - 1 - tid) : -1); };
+
+  u32x4 d[NV];
+  T edge = (T)0.f;
+  Ent<C> cur, nxt;
+  int64_t row = advance((int64_t)blockIdx.x * GPW + grp, cur.w);
+  ask_list(row, cur);
+  ask_listed_scores(row, cur);
+  if (row < a.nrows) {
+    const T* xr = (const T*)a.x + row * a.ldx;
+    const Place<T> pl(xr, a.V);
+    const int ee = edge_of(pl);
+    if (ee >= 0) edge = xr[ee];
+    const __amdgpu_buffer_rsrc_t rx = row_rsrc(xr + pl.h, pl.nmain * 16);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) d[j] = ldb16(rx, tid * 16 + j * NT * 16);
+  }
+  double v_acc = 0.0;
+  int par = 0;
+  while (row < a.nrows) {
+    const T* xr = (const T*)a.x + row * a.ldx;
+    T* gr = (T*)a.g + row * a.ldg;
+    const Place<T> pl(xr, a.V);
+    const int ee = edge_of(pl);
+    const int bbase = pl.h - BIT0;
+    const int64_t nrow = advance(row + stride, nxt.w);
+    ask_list(nrow, nxt);
+    C *lxx = lx + par * a.K, *lpp = lp + par * a.K;
+    int* lii = li + par * a.K;
+
+    // the list: its bits, classes listed twice, the teacher's maximum and sum
+    Run<C, tail, two> run;
+    run.c = c;
+    C tm = Lim<C>::lowest, ts = C(0);
+    double tmass = 0.0;
+    bool bad = cur.y == -2;
+#pragma clang loop unroll(disable)
+    for (int k = tid; k < a.K; k += NT) {
+      int id = cur.id;
+      double t = (double)cur.t;
+      C x = cur.x;
+      if (k != tid) {
+        const int64_t id64 = ld_int(a.idx, a.ibits, row * a.ldi + k);
+        id = id64 < -1 || id64 >= a.V ? -2 : (int)id64;
+        t = ld_real(a.t, a.tdt, row * a.ldt + k);
+        if (id >= 0) x = up<T>(xr[id]);
+      }
+      bad |= id == -2;
+      lii[k] = id;
+      lxx[k] = x;
+      if (id < 0) continue;
+      const int b = id - bbase;
+      const unsigned bit = 1u << (b & 31);
+      const bool first = !(atomicOr(&bm[b >> 5], bit) & bit);
+      if (!first) flags[grp][par][0] = 1;
+      if (id == cur.y) flags[grp][par][1] = 1;
+      if (tail && first) run.listed(x);
+      t *= a.invT;
+      if (tail) {
+        tmass += exp_series(t - cur.lse);
+      } else {
+        const C tc = (C)t;
+        if (tc > tm) {
+          ts *= ex2((tm - tc) * (C)LOG2E);
+          tm = tc;
+        }
+        ts += ex2((tc - tm) * (C)LOG2E);
+      }
+    }
+    if (tail) group_sync<NT>();
+    // pass 1
+    if (ee >= 0) {
+      const int b = ee - bbase;
+      const C x = up<T>(edge);
+      if (x > run.m) run.raise(x);
+      if (!(tail && ((bm[b >> 5] >> (b & 31)) & 1u))) run.s += ex2((x - run.m) * c);
+      if (two) run.s1 += ex2((x - run.m) * (C)LOG2E);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (j * NT < pl.nmain) {
+        if ((j + 1) * NT > pl.nmain && j * NT + tid >= pl.nmain) d[j] = minus_inf16<T>();
+        C f[N], e[N];
+        unpack<T>(d[j], f);
+        C vm = f[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) vm = fmx(vm, f[i]);
+        if (vm > run.m) run.raise(vm);
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = ex2((f[i] - run.m) * c);
+        if (tail) {
+          const unsigned bits = listed_bits<T>(bm, min(j * NT + tid, pl.nmain) * N + BIT0);
+          if (bits) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) e[i] = (bits >> i) & 1u ? C(0) : e[i];
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < N; o *= 2)
+#pragma unroll
+          for (int i = 0; i < N; i += 2 * o) e[i] += e[i + o];
+        run.s += e[0];
+        if (two) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) run.s1 += ex2((f[i] - run.m) * (C)LOG2E);
+        }
+      }
+    }
+    if (bad) run.s = (C)NAN;
+    // joined over the group
+    C M = wave_max(run.m);
+    C f = ex2((run.m - M) * c);
+    C s = wave_sum(run.s * f), sl = C(0), nl = C(0), s1 = C(0);
+    if (tail) sl = wave_sum(run.sl * f), nl = wave_sum(run.n);
+    if (two) s1 = wave_sum(run.s1 * ex2((run.m - M) * (C)LOG2E));
+    if (wave * 64 < a.K) {  // a wave that holds entries
+      if (tail) {
+        tmass = wave_sum(tmass);
+      } else {
+        const C wm = wave_max(tm);
+        ts = wave_sum(ts * ex2((tm - wm) * (C)LOG2E));
+        tm = wm;
+      }
+    }
+    if constexpr (NW > 1) {
+      if (lane == 0) {
+        C* o = sm[0][wave];
+        o[0] = M, o[1] = s, o[2] = sl, o[3] = s1, o[4] = nl, o[5] = tm, o[6] = ts;
+        smt[0][wave] = tmass;
+      }
+      __syncthreads();
+      const int q = (lane & 15) % NW;
+      const bool in = (lane & 15) < NW;
+      const C pm = sm[0][q][0];
+      M = row16_max(pm);
+      f = in ? ex2((pm - M) * c) : C(0);
+      s = row16_sum(in ? sm[0][q][1] * f : C(0));
+      if (tail) sl = row16_sum(in ? sm[0][q][2] * f : C(0)), nl = row16_sum(in ? sm[0][q][4] : C(0));
+      if (two) s1 = row16_sum(in ? sm[0][q][3] * ex2((pm - M) * (C)LOG2E) : C(0));
+      tm = sm[0][0][5], ts = sm[0][0][6], tmass = smt[0][0];
+#pragma clang loop unroll(disable)
+      for (int i = 1; i < NW && i * 64 < a.K; ++i) {
+        const C om = sm[0][i][5], wm = fmx(tm, om);
+        ts = ts * ex2((tm - wm) * (C)LOG2E) + sm[0][i][6] * ex2((om - wm) * (C)LOG2E);
+        tm = wm;
+        tmass += smt[0][i];
+      }
+    } else {
+      group_sync<NT>();
+    }
+    const double norm = tail ? cur.lse : uniform( (double)tm + (double)(lg2(ts) * (C)LN2));
+    const double mass = tail ? tmass : (ts == C(0) ? 0.0 : (double)(ts / ts));
+    RowScal<C> rs = row_scalars<C>(a, tail, two, cur.w, cur.y >= 0, M, s, sl, s1, nl, mass);
+    rs.M = uniform(rs.M), rs.cB = uniform(rs.cB), rs.cR = uniform(rs.cR), rs.c1 = uniform(rs.c1), rs.ql = uniform(rs.ql), rs.qy = uniform(rs.qy);
+    rs.ls = uniform(rs.ls), rs.ls1 = uniform(rs.ls1), rs.pr = uniform(rs.pr), rs.log_qr = uniform(rs.log_qr);
+    rs.empty = __builtin_amdgcn_readfirstlane(rs.empty);
+    if (tid < 2) flags[grp][par ^ 1][tid] = 0;  // the row before this one is through with them
+    ask_listed_scores(nrow, nxt);
+    // pass 2
+    const bool more = nrow < a.nrows;
+    const T* xn = (const T*)a.x + (more ? nrow : row) * a.ldx;
+    const Place<T> pn(xn, a.V);
+    const int en = edge_of(pn), next_main = more ? pn.nmain : 0;
+    const __amdgpu_buffer_rsrc_t rg = row_rsrc(gr + pl.h, pl.nmain * 16), rn = row_rsrc(xn + pn.h, next_main * 16);
+    T edge_next = (T)0.f;
+    if (more && en >= 0) edge_next = xn[en];
+    auto entry = [&](C x, C coef) { return ex2((x - rs.M) * c) * coef + (two ? ex2((x - rs.M) * (C)LOG2E) * rs.c1 : C(0)); };
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (j * NT < pl.nmain) {
+        C x[N], o[N];
+        opaque(d[j]);  // or the compiler keeps the unpacked vectors of pass 1, twice the registers
+        unpack<T>(d[j], x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = ex2((x[i] - rs.M) * c) * rs.cR;
+        if (two) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) o[i] += ex2((x[i] - rs.M) * (C)LOG2E) * rs.c1;
+        }
+        stb16(rg, tid * 16 + j * NT * 16, pack<T>(o));
+      }
+      if (j * NT < next_main) d[j] = ldb16(rn, tid * 16 + j * NT * 16);
+    }
+    if (ee >= 0) gr[ee] = (T)entry(up<T>(edge), rs.cR);
+    // the list's probabilities and its part of the value; its bits go
+#pragma clang loop unroll(disable)
+    for (int k = tid; k < a.K; k += NT) {
+      const int id = lii[k];
+      C p = C(0), l;
+      if (id >= 0) {
+        const double t = (k == tid ? (double)cur.t : ld_real(a.t, a.tdt, row * a.ldt + k)) * a.invT;
+        l = (C)(t == -INFINITY ? t : t - norm);  // (a list of -inf only has no norm)
+        p = ex2(l * (C)LOG2E);
+        if (p != C(0) && !rs.empty) v_acc += a.lam * cur.w * (double)(p * (l - ((lxx[k] - rs.M) * (C)a.invT - rs.ls)));
+        bm[(id - bbase) >> 5] = 0;
+      }
+      lpp[k] = p;
+    }
+    group_sync<NT>();  // the vectors are written: the listed entries go over them
+    const bool dup = flags[grp][par][0] != 0;
+#pragma clang loop unroll(disable)
+    for (int k = tid; k < a.K; k += NT) {
+      const int id = lii[k];
+      if (id < 0) continue;
+      C ph = lpp[k];
+      bool owner = true;
+      if (dup) {  // a class listed twice: its first entry writes the sum
+#pragma clang loop unroll(disable)
+        for (int q = 0; q < a.K; ++q) {
+          if (q == k || lii[q] != id) continue;
+          owner &= q > k;
+          ph += lpp[q];
+        }
+      }
+      if (owner) gr[id] = (T)(entry(lxx[k], rs.cB) - rs.ql * ph - (id == cur.y ? rs.qy : C(0)));
+    }
+    if (tid == NT - 1) {
+      if (cur.y >= 0) {
+        if (!flags[grp][par][1]) gr[cur.y] = (T)(entry(cur.xy, rs.cR) - rs.qy);
+        if (!rs.empty) v_acc += a.lab_lam * cur.w * (double)(rs.ls1 - (cur.xy - rs.M));
+      }
+      if (tail && rs.pr != 0.0 && !rs.empty) v_acc += a.lam * cur.w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - rs.log_qr);
+      if (rs.ls != rs.ls) v_acc = NAN;  // a NaN score, or an index or label out of range
+    }
+    edge = edge_next;
+    cur = nxt;
+    row = nrow;
+    par ^= 1;
+  }
+  double v[1] = {v_acc}, one[1] = {1.0}, fin[1];
+  if (grid_reduce_finalize<1, 0, G::WG / 64>(v, a.partials, a.counter, a.acc + 1, one, fin) && threadIdx.x == 0) {
+    *a.out = fin[0];
+    if (a.value != nullptr) *(C*)a.value = (C)fin[0];
+  }
+}
+
+template <typename T, bool tail, bool two, int NT, int NV>
+pg_status run_rows(pg_ctx* c, DArgs a, int64_t rows) {
+  using G = RowsGeom<T, NT, NV>;
+  const size_t lds = (size_t)G::group_bytes(a.V, a.K) * G::GPW;
+  a.acc = c->red_partials + PG_RED_MAX_BLOCKS;
+  a.nrows = rows;
+  int per_cu = 0;
+  void (*kernel)(DArgs) = distill_rows<T, NT, NV, tail, two>;
+  PG_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, G::WG, lds));
+  const int64_t want = (rows + G::GPW - 1) / G::GPW;
+  const int64_t grid = std::min<int64_t>(std::min<int64_t>(want, PG_RED_MAX_BLOCKS), (int64_t)std::max(per_cu, 1) * c->num_cu);
+  kernel<<<(unsigned)grid, G::WG, lds, c->stream>>>(a);
+  PG_LAUNCH_CHECK();
+  return PG_OK;
+}
+
+template <typename T, bool tail, bool two>
+pg_status run_mode(pg_ctx* c, const DArgs& a, int64_t rows) {
+  const int64_t V = a.V;
+#define PG_ROWS_TRY(NT, NV)                                                                                                              \
+  if (V <= RowsGeom<T, NT, NV>::capacity && RowsGeom<T, NT, NV>::GPW * RowsGeom<T, NT, NV>::group_bytes(a.V, a.K) <= 62 * 1024) \
+  return run_rows<T, tail, two, NT, NV>(c, a, rows)
+  PG_ROWS_TRY(64, 1);
+  PG_ROWS_TRY(64, 2);
+  PG_ROWS_TRY(64, 4);
+  PG_ROWS_TRY(64, 8);
+  PG_ROWS_TRY(256, 4);
+  PG_ROWS_TRY(256, 8);
+  PG_ROWS_TRY(256, 16);
+  PG_ROWS_TRY(512, 16);
+  PG_ROWS_TRY(1024, 16);
+#undef PG_ROWS_TRY
+  return run_parts<T, tail, two>(c, a, rows);
+}
+
+template <typename T>
+pg_status run_t(pg_ctx* c, const DArgs& a, int64_t rows) {
+  const bool tail = a.lse != nullptr && a.K > 0, two = a.lab != nullptr && a.invT != 1.0;
+  if (tail) return two ? run_mode<T, true, true>(c, a, rows) : run_mode<T, true, false>(c, a, rows);
+  return two ? run_mode<T, false, true>(c, a, rows) : run_mode<T, false, false>(c, a, rows);
+}
+
+}  // namespace
+}  // namespace pgrows

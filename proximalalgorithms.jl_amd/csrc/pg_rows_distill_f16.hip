@@ -1,0 +1,3 @@
+#include "pg_rows_distill.h"
+
+pg_status pgrows::distill_f16(pg_ctx* c, const DArgs& a, int64_t rows) { return run_t<_Float16>(c, a, rows); }
