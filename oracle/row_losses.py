@@ -77,3 +77,46 @@ def distillation(x, t, idx, *, temperature=1.0, lam=1.0, teacher_lse=None, weigh
             grad[i] += label_lam * w * (np.exp(ls) - one)
             size[i] += label_lam * w * (np.exp(ls) * (64 + 6 * far) + one)
     return float(f), grad.astype(np.float64), size.astype(np.float64), float(f_size)
+
+
+def balance(r, k, *, offsets=None, mask=None, chosen=None, lam=1.0):
+    """(f, gradient, counts, size of the gradient's terms, size of the value's terms)"""
+    r = np.asarray(r, L)
+    n, e = r.shape
+    offsets = [0, n] if offsets is None else offsets
+    mask = np.ones(n, bool) if mask is None else np.asarray(mask, bool)
+    counts = np.zeros((len(offsets) - 1, e), np.int64)
+    f, f_size = L(0), L(0)
+    grad, size = np.zeros((n, e), L), np.zeros((n, e), L)
+    for g, (a, b) in enumerate(zip(offsets, offsets[1:])):
+        tokens, bad = [t for t in range(a, b) if mask[t]], False
+        for t in tokens:
+            if chosen is not None:
+                picks = [int(c) for c in chosen[t]]
+                bad |= any(c < -1 or c >= e for c in picks)
+                picks = [c for c in picks if 0 <= c < e]
+            else:
+                order = sorted((j for j in range(e) if r[t, j] > -np.inf), key=lambda j: (-r[t, j], j))  # NaN and -inf are never chosen
+                picks = order[:k]
+            for c in picks:
+                counts[g, c] += 1
+        if not tokens:
+            continue
+        ag = L(lam) * e / (L(k) * len(tokens) ** 2)
+        c = counts[g].astype(L)
+        for t in tokens:
+            if bad or np.isnan(r[t]).any() or np.isposinf(r[t]).any():
+                f = L(np.nan)
+                grad[t] = np.nan
+                continue
+            if np.all(r[t] == -np.inf):
+                continue
+            p = np.exp(_log_softmax(r[t]))
+            far = np.where(p > 0, (r[t].max() - r[t]) / np.log(L(2)), 0.0)
+            d = (c * p).sum()
+            f += ag * d
+            spread = (c * p * (64 + 6 * far)).sum()
+            f_size += ag * (spread + 64 * d)
+            grad[t] = ag * p * (c - d)
+            size[t] = ag * p * ((c + d) * (64 + 6 * far) + spread)
+    return float(f), grad.astype(np.float64), counts, size.astype(np.float64), float(f_size)

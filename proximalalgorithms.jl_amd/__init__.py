@@ -22,7 +22,7 @@ from .operators import (Composed, Conjugate, IndAffine, IndBox, IndNonnegative, 
                         LogisticLoss, NormL1, Quadratic, SlicedSeparableSum,
                         SeparableQuadratic, SqrNormL2, SquaredDistance, Zero, convex_conjugate, gradient_, is_convex,
                         is_generalized_quadratic, prox, prox_, value_and_gradient, value_and_gradient_)
-from .row_losses import DistillationLoss
+from .row_losses import BalanceLoss, DistillationLoss
 from .panoc import PANOC, NoAcceleration, PANOCIteration, PANOCState
 from .panocplus import PANOCplus, PANOCplusIteration
 from .sharding import (NativeRcclComm, TorchDistributedComm, allreduce_sum_, attach_row_team, native_rccl_available,
@@ -39,7 +39,7 @@ from .primal_dual import (AFBA, AFBAIteration, ChambollePock, ChambollePockItera
                           AFBA_default_stepsizes)
 
 __all__ = [
-    "DistillationLoss",
+    "BalanceLoss", "DistillationLoss",
     "IndAffine", "IndNonnegative", "IndPoint", "Linear", "SlicedSeparableSum",
     "AndersonAcceleration", "AndersonAccelerationOperator", "Broyden", "BroydenOperator",
     "SFISTA", "SFISTAIteration", "DavisYin", "DavisYinIteration", "LiLin", "LiLinIteration", "DRLS", "DRLSIteration",

@@ -177,10 +177,21 @@ class pg_distill(C.Structure):
                 ("lam", C.c_double), ("label_lam", C.c_double)]
 
 
+class pg_balance_tile(C.Structure):
+    _fields_ = [("begin", C.c_int64), ("end", C.c_int64), ("group", C.c_int32), ("part", C.c_int32)]
+
+
+class pg_balance(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("groups", C.c_int64), ("ntiles", C.c_int64), ("tiles", C.c_void_p), ("mask", C.c_void_p),
+                ("chosen", C.c_void_p), ("chosen_ld", C.c_int64), ("counts", C.c_void_p), ("state", C.c_void_p), ("experts", C.c_int32),
+                ("k", C.c_int32), ("chosen_bits", C.c_int32), ("whole", C.c_int32), ("lam", C.c_double)]
+
+
 # include/proxgrad_hip_rows.h (versioned by itself; the boundary's table above stays what proxgrad_hip.h / _ext.h declare)
 PG_ROWS_ABI_VERSION = 1
 ROW_SIGNATURES = {
     "pg_distill_value_and_gradient": [_vp, C.POINTER(pg_distill), _i32, _vp, _i64, _vp, _i64, _vp, _pf64],
+    "pg_balance_value_and_gradient": [_vp, C.POINTER(pg_balance), _i32, _vp, _i64, _vp, _i64, _vp, _pf64],
 }
 
 _SPECIAL = {"pg_abi_version": ([], C.c_int32), "pg_last_error": ([], C.c_char_p), "pg_comm_available": ([], C.c_int32)}

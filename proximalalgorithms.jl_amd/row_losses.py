@@ -244,3 +244,93 @@ class DistillationLoss(_RowLoss):
     def _evaluate(self, where, value, f_out):
         up, uld, op, old, code = where
         call("pg_distill_value_and_gradient", self.ctx.handle, self._dref, code, up, uld, op, old, value, f_out)
+
+
+def _balance_tiles(tokens, offsets, num_cu):
+    """([(begin, end, group, part)], whether each group is one tile): the work of one evaluation in pieces of one group each"""
+    lengths = [b - a for a, b in zip(offsets, offsets[1:])]
+    whole = max(lengths, default=0) <= 256
+    size = max(1, max(lengths, default=0)) if whole else max(32, -(-tokens // (4 * num_cu)))
+    tiles = []
+    for g, (a, n) in enumerate(zip(offsets, lengths)):
+        parts = -(-n // size)
+        for q in range(parts):
+            tiles.append((a + n * q // parts, a + n * (q + 1) // parts, g, -1 if parts == 1 else q))
+    for a in range(offsets[-1], tokens, size):  # behind the last group
+        tiles.append((a, min(tokens, a + size), -1, 0))
+    return tiles, whole
+
+
+class BalanceLoss(_RowLoss):
+    """Balance of a router's experts (include/proxgrad_hip_rows.h: pg_balance_value_and_gradient).
+
+    The scores are a router's (tokens x n_experts), p their softmax per token; a token chooses its ``k`` highest scores (the lowest
+    index first among equal ones; never -inf), or what ``chosen`` (tokens x k; -1: none) says.  Per group g of tokens -- all of them, or
+    ``offsets[g] .. offsets[g + 1]``, a sequence each, empty ones allowed -- with c_e the choices of expert e and n the unmasked tokens:
+
+        f(u) = lam sum_g n_experts / (k n_g^2) sum_e c_ge sum_t p_te
+
+    lam per group at perfect balance.  The gradient holds the counts fixed, so f is smooth between changes of the choices only,
+    and not convex.  ``mask``: False = the token is not looked at, its gradient is zero, as behind the last group.  After an
+    evaluation ``counts`` (groups x n_experts, int32, on the device) holds the c of that evaluation: one tensor, overwritten by the next."""
+
+    is_convex = False
+
+    def __init__(self, tokens, n_experts, k, *, offsets=None, mask=None, chosen=None, lam=1.0, ctx=None):
+        torch = _torch()
+        self.rows, self.classes, self.k, self.lam = int(tokens), int(n_experts), int(k), float(lam)
+        if not 0 <= self.rows < 1 << 31:
+            raise ValueError("tokens must be between 0 and 2^31 - 1")
+        if not 1 <= self.classes <= 1024:
+            raise ValueError("n_experts must be between 1 and 1024")
+        if not 1 <= self.k <= self.classes:
+            raise ValueError("k must be between 1 and n_experts")
+        if not (self.lam >= 0 and np.isfinite(self.lam)):
+            raise ValueError("lam must be nonnegative and finite")
+        if offsets is None:
+            offsets = [0, self.rows]
+        else:
+            offsets = np.asarray(offsets.cpu() if isinstance(offsets, torch.Tensor) else offsets)
+            if offsets.ndim != 1 or offsets.size < 1:
+                raise ValueError("offsets must be a list of at least one position")
+            if offsets.dtype.kind not in "iu":
+                raise TypeError("offsets must be integers")
+            offsets = [int(o) for o in offsets]
+            if offsets[0] != 0 or offsets[-1] > self.rows or any(a > b for a, b in zip(offsets, offsets[1:])):
+                raise ValueError("offsets must start at 0, never fall, and end at most at the number of tokens")
+        if mask is not None:
+            mask = _as_tensor(mask, "mask")
+            if tuple(mask.shape) != (self.rows,):
+                raise ValueError(f"mask must have shape ({self.rows},)")
+            if mask.dtype not in (torch.bool, torch.uint8):
+                raise TypeError("mask must be boolean")
+            mask = mask.contiguous()
+        if chosen is not None:
+            chosen = _rows_of(chosen, "chosen", (self.rows, self.k), (torch.int32, torch.int64), torch.int64)
+            if not chosen.is_cuda and chosen.numel() and not (int(chosen.min()) >= -1 and int(chosen.max()) < self.classes):
+                raise ValueError("chosen must lie between -1 and n_experts - 1")
+        self.ctx = _common_device((mask, chosen), ctx)
+        dev = self.ctx.torch_device
+        groups = len(offsets) - 1
+        tiles, whole = _balance_tiles(self.rows, offsets, self.ctx.device_info()["compute_units"])
+        packed = np.array([(b, e, (g & 0xFFFFFFFF) | ((part & 0xFFFFFFFF) << 32)) for b, e, g, part in tiles], np.uint64).reshape(-1, 3).view(np.int64)
+        with _Ordered(self.ctx):
+            tiles_d = torch.from_numpy(packed).to(dev)
+            mask, chosen = (None if v is None else v.to(dev) for v in (mask, chosen))
+            self._counts = torch.zeros(groups, self.classes, dtype=torch.int32, device=dev)
+            state = torch.zeros(4 + (0 if whole else 2 * groups * (self.classes + 2)), dtype=torch.int32, device=dev)
+        self._keep = tiles_d, mask, chosen, state
+        ptr = lambda v: None if v is None else v.data_ptr()  # noqa: E731
+        self._b = _lib.pg_balance(tokens=self.rows, groups=groups, ntiles=len(tiles), tiles=ptr(tiles_d), mask=ptr(mask), chosen=ptr(chosen),
+                                  chosen_ld=0 if chosen is None else (chosen.stride(0) if self.rows > 1 else self.k), counts=ptr(self._counts),
+                                  state=ptr(state), experts=self.classes, k=self.k,
+                                  chosen_bits=64 if chosen is not None and chosen.dtype == torch.int64 else 32, whole=whole, lam=self.lam)
+        self._bref = C.byref(self._b)
+
+    @property
+    def counts(self):
+        return self._counts
+
+    def _evaluate(self, where, value, f_out):
+        up, uld, op, old, code = where
+        call("pg_balance_value_and_gradient", self.ctx.handle, self._bref, code, up, uld, op, old, value, f_out)

@@ -27,7 +27,7 @@ def test_header_and_binding_agree(tmp_path):
     lib = _lib.load()
     assert all(hasattr(lib, s) for s in declared)
     assert lib.pg_rows_abi_version() == _lib.PG_ROWS_ABI_VERSION == int(re.search(r"#define PG_ROWS_ABI_VERSION (\d+)", text).group(1))
-    structs = [("pg_distill", _lib.pg_distill)]
+    structs = [("pg_distill", _lib.pg_distill), ("pg_balance_tile", _lib.pg_balance_tile), ("pg_balance", _lib.pg_balance)]
     src = ['#include <stdio.h>', '#include <stddef.h>', '#include "proxgrad_hip_rows.h"', "int main(void) {"]
     for name, s in structs:
         src.append(f'printf("%zu\\n", sizeof({name}));')
@@ -64,12 +64,54 @@ def test_distillation_refusals():
             pa.DistillationLoss(t, i, 5)  # valid: and then there is no device, and no fallback
 
 
+def test_balance_refusals():
+    import proximalalgorithms.jl_amd as pa
+
+    bad = [
+        (ValueError, (-1, 4, 2), {}), (ValueError, (5, 0, 1), {}), (ValueError, (5, 1025, 2), {}), (ValueError, (5, 4, 0), {}), (ValueError, (5, 4, 5), {}),
+        (ValueError, (5, 4, 2), dict(lam=-1.0)), (ValueError, (5, 4, 2), dict(lam=float("inf"))), (ValueError, (1 << 31, 4, 2), {}),
+        (ValueError, (5, 4, 2), dict(offsets=[])), (ValueError, (5, 4, 2), dict(offsets=[1, 5])), (ValueError, (5, 4, 2), dict(offsets=[0, 3, 2])),
+        (ValueError, (5, 4, 2), dict(offsets=[0, 6])), (ValueError, (5, 4, 2), dict(mask=np.ones(4, bool))), (TypeError, (5, 4, 2), dict(mask=np.ones(5))),
+        (ValueError, (5, 4, 2), dict(chosen=np.zeros((5, 3), int))), (ValueError, (5, 4, 2), dict(chosen=np.full((5, 2), 4))),
+        (ValueError, (5, 4, 2), dict(chosen=np.full((5, 2), -2))), (TypeError, (5, 4, 2), dict(chosen=np.zeros((5, 2)))),
+        (TypeError, (5, 4, 2), dict(offsets=[0.0, 5.0])),
+    ]
+    for err, args, kw in bad:
+        with pytest.raises(err):
+            pa.BalanceLoss(*args, **kw)
+    if not torch.cuda.is_available():
+        with pytest.raises(pa.ProxGradError):
+            pa.BalanceLoss(5, 4, 2)
+
+
+def test_balance_tiles_cover_every_token_once():
+    from proximalalgorithms.jl_amd.row_losses import _balance_tiles
+
+    for tokens, offsets in ((0, [0, 0]), (1, [0, 1]), (5, [0, 0, 0, 4]), (1000, [0, 1, 1, 700, 999]), (100000, [0, 100000]), (4096, list(range(4097)))):
+        tiles, whole = _balance_tiles(tokens, offsets, 256)
+        seen = np.zeros(tokens, int)
+        first = set()
+        for b, e, g, part in tiles:
+            assert 0 <= b < e <= tokens and -1 <= g < len(offsets) - 1
+            seen[b:e] += 1
+            if g >= 0:
+                assert offsets[g] <= b and e <= offsets[g + 1]
+                if part <= 0:
+                    assert g not in first
+                    first.add(g)
+                assert (part == -1) == (b == offsets[g] and e == offsets[g + 1])
+        assert (seen == 1).all()
+        assert first == {g for g in range(len(offsets) - 1) if offsets[g] < offsets[g + 1]}
+        assert not whole or all(part == -1 or g < 0 for _, _, g, part in tiles)
+
+
 def test_c_entry_refuses_before_any_device_work():
     from proximalalgorithms.jl_amd import _lib
 
     lib = _lib.load()
     assert lib.pg_distill_value_and_gradient(None, None, 0, None, 0, None, 0, None, None) == _lib.PG_ERR_INVALID
     assert b"null" in lib.pg_last_error()
+    assert lib.pg_balance_value_and_gradient(None, None, 0, None, 0, None, 0, None, None) == _lib.PG_ERR_INVALID
 
 
 @pytest.mark.parametrize("rest", [False, True])
@@ -92,3 +134,20 @@ def test_oracle_distillation_gradient_is_its_differences(rest):
             xm[i, j] -= h
             d = (ref.distillation(xp, t, idx, **kw)[0] - ref.distillation(xm, t, idx, **kw)[0]) / (2 * h)
             assert abs(d - g[i, j]) < 1e-8  # second-order difference: h^2 times a third derivative of order one, plus eps / h
+
+
+def test_oracle_balance_gradient_is_its_differences():
+    rng = np.random.default_rng(4)
+    r = rng.normal(size=(9, 6))
+    kw = dict(offsets=[0, 4, 4, 8], mask=np.array([1, 1, 0, 1, 1, 1, 1, 1, 1], bool), lam=1.3)
+    f, g, counts, _, _ = ref.balance(r, 2, **kw)
+    assert counts.sum() == 2 * 7 and counts[1].sum() == 0 and not g[8].any() and not g[2].any()
+    h = 1e-5
+    for i in range(9):
+        for j in range(6):
+            rp, rm = r.copy(), r.copy()
+            rp[i, j] += h
+            rm[i, j] -= h
+            fp, fm = ref.balance(rp, 2, **kw), ref.balance(rm, 2, **kw)
+            assert np.array_equal(fp[2], counts) and np.array_equal(fm[2], counts)  # no choice changes within h
+            assert abs((fp[0] - fm[0]) / (2 * h) - g[i, j]) < 1e-8

@@ -177,3 +177,93 @@ def test_distillation_empty_and_vectors():
         assert isinstance(val, dt) and isinstance(g, m.HIPVector)
         check(torch.from_numpy(g.numpy().reshape(6, 50)), val, ref.distillation(u.reshape(6, 50), t, idx), DT["f32" if dt == np.float32 else "f64"])
         assert f(m.HIPVector.from_numpy(u)) == val
+
+
+# ---- balance ---------------------------------------------------------------------------------------------------------
+
+
+def check_balance(loss, got, value, want, dtype):
+    f, grad, counts, size, f_size = want
+    assert np.array_equal(loss.counts.cpu().numpy(), counts)
+    check(got, value, (f, grad, size, f_size), dtype)
+
+
+def router(rng, n, e, dtype, gap=0, shift=0):
+    buf = torch.full((shift + n * (e + gap),), float("nan"), dtype=dtype, device="cuda")
+    out = buf[shift:].view(n, e + gap)[:, :e]
+    out.copy_(torch.from_numpy(rng.normal(size=(n, e)) + rng.normal(size=e)))
+    return out, out.double().cpu().numpy()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n,e,k,gap,shift", [(1, 1, 1, 0, 0), (2, 4, 2, 0, 0), (7, 3, 3, 1, 1), (64, 64, 6, 0, 0), (300, 65, 8, 0, 3), (33, 127, 1, 5, 0),
+                                             (700, 128, 8, 0, 0), (20, 200, 16, 0, 1), (1500, 256, 8, 0, 0), (9, 500, 40, 3, 0), (5, 1024, 1024, 0, 0)])
+def test_balance_sizes(dtype, n, e, k, gap, shift):
+    rng = np.random.default_rng(n + e)
+    x, xe = router(rng, n, e, DT[dtype], gap, shift)
+    loss = pa().BalanceLoss(n, e, k, lam=3.0)
+    val, g = loss.value_and_gradient(x)
+    want = ref.balance(xe, k, lam=3.0)
+    check_balance(loss, g, val, want, DT[dtype])
+    for _ in range(3):  # the counts start anew each time
+        v2, g2 = loss.value_and_gradient_async(x)
+        assert torch.equal(g2, g) and float(v2) == pytest.approx(val, rel=2.0**-23)
+    assert np.array_equal(loss.counts.cpu().numpy(), want[2])
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("e,k,offsets,n", [(16, 2, [0, 1, 1, 5, 40], 40), (60, 4, [0, 0, 0], 9), (64, 6, [0, 400, 401, 900], 1000), (130, 5, list(range(0, 301, 3)), 310),
+                                           (8, 2, [0], 20)])
+def test_balance_groups_and_masks(dtype, e, k, offsets, n):
+    """ragged, empty and single-token groups, tokens behind the last one, masked tokens that hold NaN; chosen by the router itself"""
+    rng = np.random.default_rng(len(offsets) + e)
+    x, xe = router(rng, n, e, DT[dtype])
+    mask = rng.random(n) < 0.7
+    x[torch.from_numpy(~mask).cuda()] = float("nan")
+    if offsets[-1] < n:
+        x[offsets[-1]:] = float("inf")
+    xe = x.double().cpu().numpy()
+    loss = pa().BalanceLoss(n, e, k, offsets=offsets, mask=mask, lam=0.5)
+    val, g = loss.value_and_gradient(x)
+    check_balance(loss, g, val, ref.balance(xe, k, offsets=offsets, mask=mask, lam=0.5), DT[dtype])
+    chosen = rng.integers(-1, e, (n, k))
+    chosen[::3, -1] = chosen[::3, 0]  # named twice
+    for idt in (np.int32, np.int64):
+        loss = pa().BalanceLoss(n, e, k, offsets=offsets, mask=torch.from_numpy(mask).cuda(), chosen=torch.from_numpy(chosen.astype(idt)).cuda(), lam=0.5)
+        val, g = loss.value_and_gradient(x)
+        check_balance(loss, g, val, ref.balance(xe, k, offsets=offsets, mask=mask, chosen=chosen, lam=0.5), DT[dtype])
+        v2, g2 = loss.value_and_gradient_async(x, out=x.clone())
+        assert torch.equal(g2, g)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n", [9, 900])
+def test_balance_special_rows(dtype, n):
+    """equal scores, fewer live experts than k, the lowest value, NaN, infinities, a choice out of range"""
+    e, k = 70, 5
+    dt = DT[dtype]
+    rng = np.random.default_rng(1)
+    base = rng.normal(size=(n, e))
+    base[0] = 0.0  # all equal: the first five
+    base[1, 10:] = 1.0  # ties at the border
+    base[2] = -np.inf
+    base[3, 3:] = -np.inf  # three experts left
+    base[4] = torch.finfo(dt).min
+    base[5] = np.where(np.arange(e) % 3, -0.0, 0.0)  # equal in value, not in bits
+    base[6] = np.repeat(rng.normal(size=e // 2), 2)
+    base[7, :] = np.linspace(-60000, 60000, e)
+    xd = torch.from_numpy(base).to(dt).cuda()
+    loss = pa().BalanceLoss(n, e, k)
+    val, g = loss.value_and_gradient(xd)
+    check_balance(loss, g, val, ref.balance(xd.double().cpu().numpy(), k), dt)
+    xd[8, 4] = float("nan")
+    val, g = loss.value_and_gradient(xd)
+    want = ref.balance(xd.double().cpu().numpy(), k)
+    assert np.isnan(val)
+    check_balance(loss, g, val, want, dt)
+    xd[8, 4] = 0.0
+    chosen = rng.integers(0, e, (n, k))
+    chosen[n - 1, 0] = e
+    loss = pa().BalanceLoss(n, e, k, offsets=[0, n // 2, n], chosen=torch.from_numpy(chosen).cuda())
+    val, g = loss.value_and_gradient(xd)
+    check_balance(loss, g, val, ref.balance(xd.double().cpu().numpy(), k, offsets=[0, n // 2, n], chosen=chosen), dt)
