@@ -430,15 +430,8 @@ pg_status run_parts(pg_ctx* c, DArgs a, int64_t rows) {
 // NT threads hold a row as NV 16-byte vectors each (NT = 64: a wave per row, four rows per workgroup; else a workgroup per row).
 // Pass 1 takes running maximum and sums as the vectors arrive, one reduction joins them, pass 2 writes the gradient from the
 // registers and, as a vector leaves, loads the same vector of the group's NEXT row in its place, so that the memory pipes
-// stay busy through the reduction.  Loads return in order: what the next row's list needs (classes, logits, listed scores)
-// is therefore asked for before its vectors.
-template <typename C>
-struct Ent {  // of one row, per thread: entry tid of the list, the label, the teacher's normaliser, the weight
-  int id, y;  // -1 absent, -2 out of range
-  double lse, w;
-  C t, x, xy;
-};
-
+// stay busy through the reduction.  Loads return in order, so nothing may be asked for between those loads and pass 1 that
+// is needed before it: the next row's list is asked for a pass ahead and waits in LDS, and no register may spill there.
 template <typename T, int NT, int NV>
 struct RowsGeom {
   using C = typename Elem<T>::C;
@@ -447,31 +440,32 @@ struct RowsGeom {
   static constexpr int GPW = WG / NT, NW = NT / 64;
   static constexpr int capacity = NT * NV * N;  // classes a group's registers hold
   static __host__ __device__ int words(int V) { return ((V + BIT0 + N + 31) / 32 + 1) & ~1; }
-  static __host__ __device__ int group_bytes(int V, int K) {  // bitmap, then two sets (this row's, the next's) of the list's scores, probabilities, classes
-    return words(V) * 4 + (2 * K * (2 * (int)sizeof(C) + 4) + 7) / 8 * 8;
-  }
+  // two bitmaps and two lists (this row's, the next's) of scores and classes, one of logits and of probabilities
+  static __host__ __device__ int group_bytes(int V, int K) { return words(V) * 8 + (K * (4 * (int)sizeof(C) + 8) + 7) / 8 * 8; }
 };
 
 template <typename T, int NT, int NV, bool tail, bool two>
-__global__ __launch_bounds__((NT < 256 ? 256 : NT)) void distill_rows(DArgs a) {
+__global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a) {
   using G = RowsGeom<T, NT, NV>;
   using C = typename G::C;
   constexpr int N = G::N, NW = G::NW, GPW = G::GPW;
+  constexpr int AGAIN = 1 << 30;  // marks a list entry whose class an earlier one holds
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   __shared__ C sm[GPW][NW][7];
   __shared__ double smt[GPW][NW];
-  __shared__ int flags[GPW][2][2];  // [row parity][a class is listed twice, the label is listed]
+  __shared__ C sxy[GPW][2];
+  __shared__ int flags[GPW][3][2];  // [row mod 3][a class is listed twice, the label is listed]
   const int tid = threadIdx.x % NT, lane = threadIdx.x & 63;
   const int wave_in_wg = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int grp = NT == 64 ? wave_in_wg : 0, wave = NT == 64 ? 0 : wave_in_wg;
-  const int nwords = G::words(a.V);
-  unsigned* bm = (unsigned*)(lds + G::group_bytes(a.V, a.K) * grp);
-  C* lx = (C*)(bm + nwords);     // [2][K]
-  C* lp = lx + 2 * a.K;          // [2][K]
-  int* li = (int*)(lp + 2 * a.K);  // [2][K]
-#pragma clang loop unroll(disable)
-  for (int i = tid; i < nwords; i += NT) bm[i] = 0;
-  if (tid < 4) flags[grp][tid >> 1][tid & 1] = 0;
+  const int nwords = G::words(a.V), K = a.K;
+  unsigned* bm0 = (unsigned*)(lds + G::group_bytes(a.V, K) * grp);  // [2][nwords]
+  C* lx0 = (C*)(bm0 + 2 * nwords);                                  // [2][K]
+  C* lt = lx0 + 2 * K;                                              // [K] logits
+  C* lp = lt + K;                                                   // [K] probabilities
+  int* li0 = (int*)(lp + K);                                        // [2][K]
+  for (int i = tid; i < 2 * nwords; i += NT) bm0[i] = 0;
+  if (tid < 6) flags[grp][tid >> 1][tid & 1] = 0;
   group_sync<NT>();
 
   const int64_t stride = (int64_t)gridDim.x * GPW;
@@ -492,134 +486,135 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT)) void distill_rows(DArgs a) {
     }
     return row;
   };
-  auto ask_list = [&](int64_t row, Ent<C>& e) {
-    e.id = -1, e.y = -1, e.t = (C)-INFINITY, e.lse = 0.0;
+  // a row's list entry tid: class (-1 absent, -2 out of range) and logit; its label
+  auto ask_list = [&](int64_t row, int& id, C& t, int& y) {
+    id = -1, t = C(0), y = -1;
     if (row >= a.nrows) return;
-    if (tid < a.K) {
-      const int64_t id = ld_int(a.idx, a.ibits, row * a.ldi + tid);
-      e.id = id < -1 || id >= a.V ? -2 : (int)id;
-      e.t = (C)ld_real(a.t, a.tdt, row * a.ldt + tid);
+    if (tid < K) {
+      const int64_t i = ld_int(a.idx, a.ibits, row * a.ldi + tid);
+      id = i < -1 || i >= a.V ? -2 : (int)i;
+      t = (C)ld_real(a.t, a.tdt, row * a.ldt + tid);
     }
-    if (tail) e.lse = ld_real_u(a.lse, a.lsedt, row);
     if (a.lab != nullptr) {
-      const int64_t y = ld_int_u(a.lab, a.labbits, row);
-      e.y = y < -1 || y >= a.V ? -2 : (int)y;
+      const int64_t i = ld_int_u(a.lab, a.labbits, row);
+      y = i < -1 || i >= a.V ? -2 : (int)i;
     }
   };
-  auto ask_listed_scores = [&](int64_t row, Ent<C>& e) {
-    e.x = e.xy = Lim<C>::lowest;
+  // ... and the scores there (before anything overwrites them: the gradient may go into the scores' buffer)
+  auto ask_scores = [&](int64_t row, int id, int y, C& x, C& xy) {
+    x = xy = C(0);
     if (row >= a.nrows) return;
     const T* xr = (const T*)a.x + row * a.ldx;
-    if (e.id >= 0) e.x = up<T>(xr[e.id]);
-    if (e.y >= 0) e.xy = up<T>(xr[e.y]);
+    if (id >= 0) x = up<T>(xr[id]);
+    if (y >= 0 && tid == NT - 1) xy = up<T>(xr[y]);
+  };
+  // the list into LDS: classes and their bits, scores, logits
+  auto put_list = [&](int64_t row, int id, C t, int y, C x, C xy, int par, int slot) {
+    if (row >= a.nrows) return;
+    const T* xr = (const T*)a.x + row * a.ldx;
+    const Place<T> pl(xr, a.V);
+    unsigned* bm = bm0 + par * nwords;
+#pragma clang loop unroll(disable)
+    for (int k = tid; k < K; k += NT) {
+      if (k != tid) {
+        const int64_t i = ld_int(a.idx, a.ibits, row * a.ldi + k);
+        id = i < -1 || i >= a.V ? -2 : (int)i;
+        t = (C)ld_real(a.t, a.tdt, row * a.ldt + k);
+        if (id >= 0) x = up<T>(xr[id]);
+      }
+      int mark = 0;
+      if (id >= 0) {
+        const int b = id - pl.h + BIT0;
+        const unsigned bit = 1u << (b & 31);
+        if (atomicOr(&bm[b >> 5], bit) & bit) {
+          mark = AGAIN;
+          flags[grp][slot][0] = 1;
+        }
+        if (id == y) flags[grp][slot][1] = 1;
+      }
+      li0[par * K + k] = id < 0 ? id : id | mark;
+      lx0[par * K + k] = x;
+      lt[k] = t;
+    }
+    if (tid == NT - 1) sxy[grp][par] = xy;
   };
   // head elements: threads 0 ..; tail elements: threads NT - 1 .. down
   auto edge_of = [&](const Place<T>& pl) { return tid < pl.h ? tid : (pl.hV + (NT - 1 - tid) < a.V ? pl.hV + (NT - 1 - tid) : -1); };
 
   u32x4 d[NV];
   T edge = (T)0.f;
-  Ent<C> cur, nxt;
-  int64_t row = advance((int64_t)blockIdx.x * GPW + grp, cur.w);
-  ask_list(row, cur);
-  ask_listed_scores(row, cur);
-  if (row < a.nrows) {
-    const T* xr = (const T*)a.x + row * a.ldx;
-    const Place<T> pl(xr, a.V);
-    const int ee = edge_of(pl);
-    if (ee >= 0) edge = xr[ee];
-    const __amdgpu_buffer_rsrc_t rx = row_rsrc(xr + pl.h, pl.nmain * 16);
+  double w;
+  int y, par = 0, slot = 0;
+  int64_t row = advance((int64_t)blockIdx.x * GPW + grp, w);
+  {
+    int id;
+    C t, x, xy;
+    ask_list(row, id, t, y);
+    ask_scores(row, id, y, x, xy);
+    if (row < a.nrows) {
+      const T* xr = (const T*)a.x + row * a.ldx;
+      const Place<T> pl(xr, a.V);
+      const int ee = edge_of(pl);
+      if (ee >= 0) edge = xr[ee];
+      const __amdgpu_buffer_rsrc_t rx = row_rsrc(xr + pl.h, pl.nmain * 16);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) d[j] = ldb16(rx, tid * 16 + j * NT * 16);
+      for (int j = 0; j < NV; ++j) d[j] = ldb16(rx, tid * 16 + j * NT * 16);
+    }
+    put_list(row, id, t, y, x, xy, 0, 0);
+    group_sync<NT>();
   }
   double v_acc = 0.0;
-  int par = 0;
   while (row < a.nrows) {
     const T* xr = (const T*)a.x + row * a.ldx;
     T* gr = (T*)a.g + row * a.ldg;
     const Place<T> pl(xr, a.V);
     const int ee = edge_of(pl);
     const int bbase = pl.h - BIT0;
-    const int64_t nrow = advance(row + stride, nxt.w);
-    ask_list(nrow, nxt);
-    C *lxx = lx + par * a.K, *lpp = lp + par * a.K;
-    int* lii = li + par * a.K;
+    unsigned* bm = bm0 + par * nwords;
+    const C* lx = lx0 + par * K;
+    const int* li = li0 + par * K;
+    double w_next;
+    int id_next, y_next;
+    C t_next;
+    const int64_t nrow = advance(row + stride, w_next);
+    ask_list(nrow, id_next, t_next, y_next);
 
-    // the list: its bits, classes listed twice, the teacher's maximum and sum
+    // pass 1
     Run<C, tail, two> run;
     run.c = c;
-    C tm = Lim<C>::lowest, ts = C(0);
-    double tmass = 0.0;
-    bool bad = cur.y == -2;
-#pragma clang loop unroll(disable)
-    for (int k = tid; k < a.K; k += NT) {
-      int id = cur.id;
-      double t = (double)cur.t;
-      C x = cur.x;
-      if (k != tid) {
-        const int64_t id64 = ld_int(a.idx, a.ibits, row * a.ldi + k);
-        id = id64 < -1 || id64 >= a.V ? -2 : (int)id64;
-        t = ld_real(a.t, a.tdt, row * a.ldt + k);
-        if (id >= 0) x = up<T>(xr[id]);
-      }
-      bad |= id == -2;
-      lii[k] = id;
-      lxx[k] = x;
-      if (id < 0) continue;
-      const int b = id - bbase;
-      const unsigned bit = 1u << (b & 31);
-      const bool first = !(atomicOr(&bm[b >> 5], bit) & bit);
-      if (!first) flags[grp][par][0] = 1;
-      if (id == cur.y) flags[grp][par][1] = 1;
-      if (tail && first) run.listed(x);
-      t *= a.invT;
-      if (tail) {
-        tmass += exp_series(t - cur.lse);
-      } else {
-        const C tc = (C)t;
-        if (tc > tm) {
-          ts *= ex2((tm - tc) * (C)LOG2E);
-          tm = tc;
-        }
-        ts += ex2((tc - tm) * (C)LOG2E);
-      }
-    }
-    if (tail) group_sync<NT>();
-    // pass 1
-    if (ee >= 0) {
-      const int b = ee - bbase;
-      const C x = up<T>(edge);
-      if (x > run.m) run.raise(x);
-      if (!(tail && ((bm[b >> 5] >> (b & 31)) & 1u))) run.s += ex2((x - run.m) * c);
-      if (two) run.s1 += ex2((x - run.m) * (C)LOG2E);
-    }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (j * NT < pl.nmain) {
         if ((j + 1) * NT > pl.nmain && j * NT + tid >= pl.nmain) d[j] = minus_inf16<T>();
-        C f[N], e[N];
+        C f[N];
         unpack<T>(d[j], f);
-        C vm = f[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) vm = fmx(vm, f[i]);
-        if (vm > run.m) run.raise(vm);
-#pragma unroll
-        for (int i = 0; i < N; ++i) e[i] = ex2((f[i] - run.m) * c);
-        if (tail) {
-          const unsigned bits = listed_bits<T>(bm, min(j * NT + tid, pl.nmain) * N + BIT0);
-          if (bits) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) e[i] = (bits >> i) & 1u ? C(0) : e[i];
-          }
+        run.template add<N>(f, tail ? listed_bits<T>(bm, min(j * NT + tid, pl.nmain) * N + BIT0) : 0u);
+      }
+    }
+    if (ee >= 0) {
+      const int b = ee - bbase;
+      run.add1(up<T>(edge), tail && ((bm[b >> 5] >> (b & 31)) & 1u));
+    }
+    // the list: the teacher's maximum and sum, the scores the sums have left out
+    C tm = Lim<C>::lowest, ts = C(0);
+    double tmass = 0.0;
+    bool bad = y == -2;
+    const double lse = tail ? ld_real_u(a.lse, a.lsedt, row) : 0.0;
+#pragma clang loop unroll(disable)
+    for (int k = tid; k < K; k += NT) {
+      const int id = li[k];
+      bad |= id == -2;
+      if (id < 0) continue;
+      if constexpr (tail) {
+        if (!(id & AGAIN)) run.listed(lx[k]);
+        tmass += exp_series((double)lt[k] * a.invT - lse);
+      } else {
+        const C t = (C)((double)lt[k] * a.invT);
+        if (t > tm) {
+          ts *= ex2((tm - t) * (C)LOG2E);
+          tm = t;
         }
-#pragma unroll
-        for (int o = 1; o < N; o *= 2)
-#pragma unroll
-          for (int i = 0; i < N; i += 2 * o) e[i] += e[i + o];
-        run.s += e[0];
-        if (two) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) run.s1 += ex2((f[i] - run.m) * (C)LOG2E);
-        }
+        ts += ex2((t - tm) * (C)LOG2E);
       }
     }
     if (bad) run.s = (C)NAN;
@@ -627,10 +622,10 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT)) void distill_rows(DArgs a) {
     C M = wave_max(run.m);
     C f = ex2((run.m - M) * c);
     C s = wave_sum(run.s * f), sl = C(0), nl = C(0), s1 = C(0);
-    if (tail) sl = wave_sum(run.sl * f), nl = wave_sum(run.n);
-    if (two) s1 = wave_sum(run.s1 * ex2((run.m - M) * (C)LOG2E));
-    if (wave * 64 < a.K) {  // a wave that holds entries
-      if (tail) {
+    if constexpr (tail) sl = wave_sum(run.sl * f), nl = wave_sum(run.n);
+    if constexpr (two) s1 = wave_sum(run.s1 * ex2((run.m - M) * (C)LOG2E));
+    if (wave * 64 < K) {  // a wave that holds entries
+      if constexpr (tail) {
         tmass = wave_sum(tmass);
       } else {
         const C wm = wave_max(tm);
@@ -651,27 +646,32 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT)) void distill_rows(DArgs a) {
       M = row16_max(pm);
       f = in ? ex2((pm - M) * c) : C(0);
       s = row16_sum(in ? sm[0][q][1] * f : C(0));
-      if (tail) sl = row16_sum(in ? sm[0][q][2] * f : C(0)), nl = row16_sum(in ? sm[0][q][4] : C(0));
-      if (two) s1 = row16_sum(in ? sm[0][q][3] * ex2((pm - M) * (C)LOG2E) : C(0));
+      if constexpr (tail) sl = row16_sum(in ? sm[0][q][2] * f : C(0)), nl = row16_sum(in ? sm[0][q][4] : C(0));
+      if constexpr (two) s1 = row16_sum(in ? sm[0][q][3] * ex2((pm - M) * (C)LOG2E) : C(0));
       tm = sm[0][0][5], ts = sm[0][0][6], tmass = smt[0][0];
 #pragma clang loop unroll(disable)
-      for (int i = 1; i < NW && i * 64 < a.K; ++i) {
-        const C om = sm[0][i][5], wm = fmx(tm, om);
-        ts = ts * ex2((tm - wm) * (C)LOG2E) + sm[0][i][6] * ex2((om - wm) * (C)LOG2E);
-        tm = wm;
-        tmass += smt[0][i];
+      for (int i = 1; i < NW && i * 64 < K; ++i) {
+        if constexpr (tail) {
+          tmass += smt[0][i];
+        } else {
+          const C om = sm[0][i][5], wm = fmx(tm, om);
+          ts = ts * ex2((tm - wm) * (C)LOG2E) + sm[0][i][6] * ex2((om - wm) * (C)LOG2E);
+          tm = wm;
+        }
       }
     } else {
       group_sync<NT>();
     }
-    const double norm = tail ? cur.lse : uniform( (double)tm + (double)(lg2(ts) * (C)LN2));
+    const double norm = tail ? lse : uniform((double)tm + (double)(lg2(ts) * (C)LN2));
     const double mass = tail ? tmass : (ts == C(0) ? 0.0 : (double)(ts / ts));
-    RowScal<C> rs = row_scalars<C>(a, tail, two, cur.w, cur.y >= 0, M, s, sl, s1, nl, mass);
+    RowScal<C> rs = row_scalars<C>(a, tail, two, w, y >= 0, M, s, sl, s1, nl, mass);
     rs.M = uniform(rs.M), rs.cB = uniform(rs.cB), rs.cR = uniform(rs.cR), rs.c1 = uniform(rs.c1), rs.ql = uniform(rs.ql), rs.qy = uniform(rs.qy);
     rs.ls = uniform(rs.ls), rs.ls1 = uniform(rs.ls1), rs.pr = uniform(rs.pr), rs.log_qr = uniform(rs.log_qr);
     rs.empty = __builtin_amdgcn_readfirstlane(rs.empty);
-    if (tid < 2) flags[grp][par ^ 1][tid] = 0;  // the row before this one is through with them
-    ask_listed_scores(nrow, nxt);
+    const int slot_next = slot == 2 ? 0 : slot + 1;
+    if (tid < 2) flags[grp][slot_next == 2 ? 0 : slot_next + 1][tid] = 0;  // the row before this one is through with them
+    C x_next, xy_next;
+    ask_scores(nrow, id_next, y_next, x_next, xy_next);
     // pass 2
     const bool more = nrow < a.nrows;
     const T* xn = (const T*)a.x + (more ? nrow : row) * a.ldx;
@@ -689,7 +689,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT)) void distill_rows(DArgs a) {
         unpack<T>(d[j], x);
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i] = ex2((x[i] - rs.M) * c) * rs.cR;
-        if (two) {
+        if constexpr (two) {
 #pragma unroll
           for (int i = 0; i < N; ++i) o[i] += ex2((x[i] - rs.M) * (C)LOG2E) * rs.c1;
         }
@@ -700,48 +700,48 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT)) void distill_rows(DArgs a) {
     if (ee >= 0) gr[ee] = (T)entry(up<T>(edge), rs.cR);
     // the list's probabilities and its part of the value; its bits go
 #pragma clang loop unroll(disable)
-    for (int k = tid; k < a.K; k += NT) {
-      const int id = lii[k];
-      C p = C(0), l;
+    for (int k = tid; k < K; k += NT) {
+      const int id = li[k];
+      C p = C(0);
       if (id >= 0) {
-        const double t = (k == tid ? (double)cur.t : ld_real(a.t, a.tdt, row * a.ldt + k)) * a.invT;
-        l = (C)(t == -INFINITY ? t : t - norm);  // (a list of -inf only has no norm)
+        const double t = (double)lt[k] * a.invT;
+        const C l = t == -INFINITY ? (C)t : (C)(t - norm);  // (a list of -inf only has no norm)
         p = ex2(l * (C)LOG2E);
-        if (p != C(0) && !rs.empty) v_acc += a.lam * cur.w * (double)(p * (l - ((lxx[k] - rs.M) * (C)a.invT - rs.ls)));
-        bm[(id - bbase) >> 5] = 0;
+        if (p != C(0) && !rs.empty) v_acc += a.lam * w * (double)(p * (l - ((lx[k] - rs.M) * (C)a.invT - rs.ls)));
+        bm[((id & ~AGAIN) - bbase) >> 5] = 0;
       }
-      lpp[k] = p;
+      lp[k] = p;
     }
+    put_list(nrow, id_next, t_next, y_next, x_next, xy_next, par ^ 1, slot_next);
     group_sync<NT>();  // the vectors are written: the listed entries go over them
-    const bool dup = flags[grp][par][0] != 0;
+    const bool dup = flags[grp][slot][0] != 0;
 #pragma clang loop unroll(disable)
-    for (int k = tid; k < a.K; k += NT) {
-      const int id = lii[k];
-      if (id < 0) continue;
-      C ph = lpp[k];
-      bool owner = true;
-      if (dup) {  // a class listed twice: its first entry writes the sum
+    for (int k = tid; k < K; k += NT) {
+      const int id = li[k];
+      if (id < 0 || (id & AGAIN)) continue;
+      C ph = lp[k];
+      if (dup) {  // a class listed twice: the entry that holds it writes the sum
 #pragma clang loop unroll(disable)
-        for (int q = 0; q < a.K; ++q) {
-          if (q == k || lii[q] != id) continue;
-          owner &= q > k;
-          ph += lpp[q];
-        }
+        for (int q = 0; q < K; ++q)
+          if (li[q] == (id | AGAIN)) ph += lp[q];
       }
-      if (owner) gr[id] = (T)(entry(lxx[k], rs.cB) - rs.ql * ph - (id == cur.y ? rs.qy : C(0)));
+      gr[id] = (T)(entry(lx[k], rs.cB) - rs.ql * ph - (id == y ? rs.qy : C(0)));
     }
     if (tid == NT - 1) {
-      if (cur.y >= 0) {
-        if (!flags[grp][par][1]) gr[cur.y] = (T)(entry(cur.xy, rs.cR) - rs.qy);
-        if (!rs.empty) v_acc += a.lab_lam * cur.w * (double)(rs.ls1 - (cur.xy - rs.M));
+      if (y >= 0) {
+        const C xy = sxy[grp][par];
+        if (!flags[grp][slot][1]) gr[y] = (T)(entry(xy, rs.cR) - rs.qy);
+        if (!rs.empty) v_acc += a.lab_lam * w * (double)(rs.ls1 - (xy - rs.M));
       }
-      if (tail && rs.pr != 0.0 && !rs.empty) v_acc += a.lam * cur.w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - rs.log_qr);
+      if (tail && rs.pr != 0.0 && !rs.empty) v_acc += a.lam * w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - rs.log_qr);
       if (rs.ls != rs.ls) v_acc = NAN;  // a NaN score, or an index or label out of range
     }
     edge = edge_next;
-    cur = nxt;
+    y = y_next;
+    w = w_next;
     row = nrow;
     par ^= 1;
+    slot = slot_next;
   }
   double v[1] = {v_acc}, one[1] = {1.0}, fin[1];
   if (grid_reduce_finalize<1, 0, G::WG / 64>(v, a.partials, a.counter, a.acc + 1, one, fin) && threadIdx.x == 0) {
