@@ -93,7 +93,7 @@ __device__ __forceinline__ void st16(T* p, u32x4 v) {
 // vector v of a row: a wave-uniform base and a 32-bit offset (a row is at most 2^30 elements of at most 8 bytes: the product is unsigned)
 template <typename T>
 __device__ __forceinline__ T* at16(T* base, int v) {
-  return (T*)((uintptr_t)base + (uint64_t)(unsigned)v * 16u);
+  return (T*)((const char*)base + (uint64_t)(unsigned)v * 16u);  // (through char*: an integer would lose the address space)
 }
 // A row as a buffer resource: base and length in scalar registers, one 32-bit offset per lane; a load behind the end gives 0, a
 // store behind it is dropped (the hardware's bounds check), so no vector needs a mask or a 64-bit address of its own.
@@ -111,6 +111,9 @@ __device__ __forceinline__ u32x4 minus_inf16() {
   return __builtin_bit_cast(u32x4, e);
 }
 // a value the compiler knows nothing about any more
+__device__ __forceinline__ void opaque(int& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void opaque(float& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void opaque(double& v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void opaque(u32x4& v) { asm volatile("" : "+v"(v)); }
 template <typename T>
 __device__ __forceinline__ void unpack(u32x4 u, typename Elem<T>::C (&f)[Elem<T>::N]) {
@@ -135,6 +138,39 @@ __device__ __forceinline__ double ld_real(const void* p, int dt, int64_t i) {
     default: return (double)(float)((const _Float16*)p)[i];
   }
 }
+// the same in two steps: loads whose results nothing looks at yet (a conversion beside them would wait for them, and so would two
+// kinds of load into one register), and the conversion.  Two loads each, whatever the type: of the element's halves, or twice the same
+template <typename C>
+struct RawReal {  // C = float: of 2 or 4 bytes; C = double: of 8
+  unsigned a, b;
+  __device__ __forceinline__ void load(const void* p, int dt, int64_t i) {
+    if constexpr (sizeof(C) == 8) {
+      const uint2 v = ((const uint2*)p)[i];
+      a = v.x, b = v.y;
+    } else {
+      const int h = dt == PG_F32 ? 1 : 0;  // halves behind the first
+      const unsigned short* q = (const unsigned short*)p + (i << h);
+      a = q[0], b = q[h];
+    }
+  }
+  __device__ __forceinline__ C get(int dt) const {
+    if constexpr (sizeof(C) == 8) {
+      return __builtin_bit_cast(double, make_uint2(a, b));
+    } else {
+      return dt == PG_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)a) : __builtin_bit_cast(float, dt == PG_F32 ? a | b << 16 : a << 16);
+    }
+  }
+  static bool takes(int dt) { return (dt == PG_F64) == (sizeof(C) == 8); }
+};
+struct RawInt {
+  unsigned a, b;
+  __device__ __forceinline__ void load(const void* p, int bits, int64_t i) {
+    const int h = bits == 64 ? 1 : 0;
+    const unsigned* q = (const unsigned*)p + (i << h);
+    a = q[0], b = q[h];
+  }
+  __device__ __forceinline__ int64_t get(int bits) const { return bits == 64 ? (int64_t)(((unsigned long long)b << 32) | a) : (int64_t)(int)a; }
+};
 __device__ __forceinline__ int64_t ld_int(const void* p, int bits, int64_t i) {
   return bits == 64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
 }

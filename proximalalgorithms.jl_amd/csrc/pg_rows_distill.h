@@ -54,8 +54,8 @@ struct RowScal {
   double pr, log_qr;
   bool empty;
 };
-template <typename C>
-__device__ __forceinline__ RowScal<C> row_scalars(const DArgs& a, bool tail, bool two, double w, bool has_label, C M, C s_rest, C s_list, C s1,
+template <typename C, typename Args>
+__device__ __forceinline__ RowScal<C> row_scalars(const Args& a, bool tail, bool two, double w, bool has_label, C M, C s_rest, C s_list, C s1,
                                                   C n_listed, double mass) {
   RowScal<C> r;
   const C S = tail ? s_rest + s_list : s_rest;
@@ -123,11 +123,13 @@ __device__ __forceinline__ unsigned listed_bits(const unsigned* bm, int vbit) { 
   return (bm[vbit >> 5] >> (vbit & 31)) & ((1u << N) - 1u);
 }
 
-// running maximum and sums of one thread
+// Sums of one thread, relative to a reference score m that is one of the row's (or the type's lowest value while there is
+// none): any score will do that is no more than 59 powers of two (41 = 59 ln 2) below the largest, so m is raised rarely, by a branch.
 template <typename C, bool TAIL, bool TWO>
 struct Run {
-  C m = Lim<C>::lowest, s = C(0), sl = C(0), s1 = C(0), n = C(0);
-  C c;  // log2(e) / T
+  C m = Lim<C>::lowest, lim = Lim<C>::lowest, s = C(0), sl = C(0), s1 = C(0), n = C(0);
+  C c, head;  // log2(e) / T; 59 powers of two in scores
+  __device__ __forceinline__ explicit Run(double invT) : c(uniform((C)(invT * LOG2E))), head(uniform((C)(41.0 / fmax(invT, 1.0)))) {}
   __device__ __forceinline__ void raise(C to) {
     const C d = m - to;
     const C f = ex2(d * c);
@@ -135,9 +137,11 @@ struct Run {
     if constexpr (TAIL) sl *= f;
     if constexpr (TWO) s1 *= ex2(d * (C)LOG2E);
     m = to;
+    lim = to + head;
+    opaque(m);  // keep the branch
   }
   __device__ __forceinline__ void listed(C x) {  // a listed class (TAIL only)
-    if (x > m) raise(x);
+    if (x > lim) raise(x);
     sl += ex2((x - m) * c);
     n += C(1);
   }
@@ -146,10 +150,20 @@ struct Run {
     C vm = f[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) vm = fmx(vm, f[i]);
-    if (vm > m) raise(vm);
+    if (vm > lim) raise(vm);
     C e[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) e[i] = ex2((f[i] - m) * c);
+    if constexpr (TWO) {
+      C t[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) t[i] = ex2((f[i] - m) * (C)LOG2E);
+#pragma unroll
+      for (int o = 1; o < N; o *= 2)
+#pragma unroll
+        for (int i = 0; i < N; i += 2 * o) t[i] += t[i + o];
+      s1 += t[0];
+    }
     if constexpr (TAIL) {
       if (bits) {
 #pragma unroll
@@ -161,15 +175,9 @@ struct Run {
 #pragma unroll
       for (int i = 0; i < N; i += 2 * o) e[i] += e[i + o];
     s += e[0];
-    if constexpr (TWO) {
-      C t = C(0);
-#pragma unroll
-      for (int i = 0; i < N; ++i) t += ex2((f[i] - m) * (C)LOG2E);
-      s1 += t;
-    }
   }
   __device__ __forceinline__ void add1(C x, bool in_list) {
-    if (x > m) raise(x);
+    if (x > lim) raise(x);
     if (!(TAIL && in_list)) s += ex2((x - m) * c);
     if constexpr (TWO) s1 += ex2((x - m) * (C)LOG2E);
   }
@@ -201,8 +209,7 @@ __global__ __launch_bounds__(PT) void distill_part_stats(DArgs a) {
     for (int i = tid; i < words; i += PT) bm[i] = 0;
     __syncthreads();
   }
-  Run<C, TAIL, TWO> run;
-  run.c = (C)(a.invT * LOG2E);
+  Run<C, TAIL, TWO> run(a.invT);
   bool bad = false;
   for (int k = tid; k < a.K; k += PT) {
     const int64_t id = ld_int(a.idx, a.ibits, row * a.ldi + k);
@@ -445,7 +452,11 @@ struct RowsGeom {
 };
 
 template <typename T, int NT, int NV, bool tail, bool two>
-__global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a) {
+__global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) {
+  // The arguments stay in memory and are read where they are used: hoisted out of the row loop they fill the scalar registers and
+  // spill into vector ones
+  const PG_CONST_AS DArgs* ap = (const PG_CONST_AS DArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+#define a (*ap)
   using G = RowsGeom<T, NT, NV>;
   using C = typename G::C;
   constexpr int N = G::N, NW = G::NW, GPW = G::GPW;
@@ -469,8 +480,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a
   group_sync<NT>();
 
   const int64_t stride = (int64_t)gridDim.x * GPW;
-  const C c = (C)(a.invT * LOG2E);
-  const u32x4 zero = {0u, 0u, 0u, 0u};
+  const C c = uniform((C)(a.invT * LOG2E));
 
   // the next row that has a weight (the others' gradients are zeros)
   auto advance = [&](int64_t row, double& w) {
@@ -479,6 +489,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a
       if (a.w == nullptr || (w = ld_real_u(a.w, a.wdt, row)) != 0.0) break;
       T* gr = (T*)a.g + row * a.ldg;
       const Place<T> pl(gr, a.V);
+      const u32x4 zero = {0u, 0u, 0u, 0u};
 #pragma clang loop unroll(disable)
       for (int v = tid; v < pl.nmain; v += NT) st16(at16(gr + pl.h, v), zero);
       if (tid < pl.h) gr[tid] = (T)0.f;
@@ -486,42 +497,35 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a
     }
     return row;
   };
-  // a row's list entry tid: class (-1 absent, -2 out of range) and logit; its label
-  auto ask_list = [&](int64_t row, int& id, C& t, int& y) {
-    id = -1, t = C(0), y = -1;
-    if (row >= a.nrows) return;
-    if (tid < K) {
-      const int64_t i = ld_int(a.idx, a.ibits, row * a.ldi + tid);
-      id = i < -1 || i >= a.V ? -2 : (int)i;
-      t = (C)ld_real(a.t, a.tdt, row * a.ldt + tid);
-    }
-    if (a.lab != nullptr) {
-      const int64_t i = ld_int_u(a.lab, a.labbits, row);
-      y = i < -1 || i >= a.V ? -2 : (int)i;
+  // a row's list entry tid (class, logit) and label, not looked at yet
+  auto ask_list = [&](int64_t row, RawInt& id, RawReal<C>& t, int64_t& y) {
+    y = -1;
+    if (row < a.nrows) {
+      if (tid < K) {
+        id.load(a.idx, a.ibits, row * a.ldi + tid);
+        t.load(a.t, a.tdt, row * a.ldt + tid);
+      }
+      if (a.lab != nullptr) y = ld_int_u(a.lab, a.labbits, row);
     }
   };
+  // class or label: -1 absent, -2 out of range
+  auto checked = [&](int64_t i) { return i < -1 || i >= a.V ? -2 : (int)i; };
   // ... and the scores there (before anything overwrites them: the gradient may go into the scores' buffer)
-  auto ask_scores = [&](int64_t row, int id, int y, C& x, C& xy) {
-    x = xy = C(0);
-    if (row >= a.nrows) return;
-    const T* xr = (const T*)a.x + row * a.ldx;
-    if (id >= 0) x = up<T>(xr[id]);
-    if (y >= 0 && tid == NT - 1) xy = up<T>(xr[y]);
+  auto ask_scores = [&](int64_t row, int id, int y, T& x, T& xy) {
+    x = xy = (T)0.f;
+    if (row < a.nrows) {
+      const T* xr = (const T*)a.x + row * a.ldx;
+      if (id >= 0) x = xr[id];
+      if (y >= 0 && tid == NT - 1) xy = xr[y];
+    }
   };
   // the list into LDS: classes and their bits, scores, logits
-  auto put_list = [&](int64_t row, int id, C t, int y, C x, C xy, int par, int slot) {
+  auto put_list = [&](int64_t row, int id, RawReal<C> t, int y, T x, T xy, int par, int slot) {
     if (row >= a.nrows) return;
     const T* xr = (const T*)a.x + row * a.ldx;
     const Place<T> pl(xr, a.V);
     unsigned* bm = bm0 + par * nwords;
-#pragma clang loop unroll(disable)
-    for (int k = tid; k < K; k += NT) {
-      if (k != tid) {
-        const int64_t i = ld_int(a.idx, a.ibits, row * a.ldi + k);
-        id = i < -1 || i >= a.V ? -2 : (int)i;
-        t = (C)ld_real(a.t, a.tdt, row * a.ldt + k);
-        if (id >= 0) x = up<T>(xr[id]);
-      }
+    auto put = [&](int k, int id, C t, T x) {
       int mark = 0;
       if (id >= 0) {
         const int b = id - pl.h + BIT0;
@@ -533,10 +537,16 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a
         if (id == y) flags[grp][slot][1] = 1;
       }
       li0[par * K + k] = id < 0 ? id : id | mark;
-      lx0[par * K + k] = x;
+      lx0[par * K + k] = up<T>(x);
       lt[k] = t;
+    };
+    if (tid < K) put(tid, id, t.get(a.tdt), x);
+#pragma clang loop unroll(disable)
+    for (int k = tid + NT; k < K; k += NT) {
+      const int i = checked(ld_int(a.idx, a.ibits, row * a.ldi + k));
+      put(k, i, (C)ld_real(a.t, a.tdt, row * a.ldt + k), i >= 0 ? xr[i] : (T)0.f);
     }
-    if (tid == NT - 1) sxy[grp][par] = xy;
+    if (tid == NT - 1) sxy[grp][par] = up<T>(xy);
   };
   // head elements: threads 0 ..; tail elements: threads NT - 1 .. down
   auto edge_of = [&](const Place<T>& pl) { return tid < pl.h ? tid : (pl.hV + (NT - 1 - tid) < a.V ? pl.hV + (NT - 1 - tid) : -1); };
@@ -547,9 +557,13 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a
   int y, par = 0, slot = 0;
   int64_t row = advance((int64_t)blockIdx.x * GPW + grp, w);
   {
-    int id;
-    C t, x, xy;
-    ask_list(row, id, t, y);
+    RawInt rid;
+    RawReal<C> t;
+    T x, xy;
+    int64_t ry;
+    ask_list(row, rid, t, ry);
+    const int id = row < a.nrows && tid < K ? checked(rid.get(a.ibits)) : -1;
+    y = checked(ry);
     ask_scores(row, id, y, x, xy);
     if (row < a.nrows) {
       const T* xr = (const T*)a.x + row * a.ldx;
@@ -557,14 +571,16 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a
       const int ee = edge_of(pl);
       if (ee >= 0) edge = xr[ee];
       const __amdgpu_buffer_rsrc_t rx = row_rsrc(xr + pl.h, pl.nmain * 16);
+      const int off = tid * 16;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) d[j] = ldb16(rx, tid * 16 + j * NT * 16);
+      for (int j = 0; j < NV; ++j) d[j] = ldb16(rx, off + j * NT * 16);
     }
     put_list(row, id, t, y, x, xy, 0, 0);
     group_sync<NT>();
   }
   double v_acc = 0.0;
   while (row < a.nrows) {
+    asm volatile("" : "+s"(ap));
     const T* xr = (const T*)a.x + row * a.ldx;
     T* gr = (T*)a.g + row * a.ldg;
     const Place<T> pl(xr, a.V);
@@ -574,21 +590,26 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a
     const C* lx = lx0 + par * K;
     const int* li = li0 + par * K;
     double w_next;
-    int id_next, y_next;
-    C t_next;
+    RawInt id_raw;
+    RawReal<C> t_next;
+    int64_t y_raw;
     const int64_t nrow = advance(row + stride, w_next);
-    ask_list(nrow, id_next, t_next, y_next);
+    ask_list(nrow, id_raw, t_next, y_raw);
 
     // pass 1
-    Run<C, tail, two> run;
-    run.c = c;
+    Run<C, tail, two> run(a.invT);
+    int t0 = tid;
+    opaque(t0);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (j * NT < pl.nmain) {
-        if ((j + 1) * NT > pl.nmain && j * NT + tid >= pl.nmain) d[j] = minus_inf16<T>();
+        if ((j + 1) * NT > pl.nmain) {
+          if (j * NT + t0 >= pl.nmain) d[j] = minus_inf16<T>();
+          opaque(d[j]);  // keep the branch: every vector but one is whole
+        }
         C f[N];
         unpack<T>(d[j], f);
-        run.template add<N>(f, tail ? listed_bits<T>(bm, min(j * NT + tid, pl.nmain) * N + BIT0) : 0u);
+        run.template add<N>(f, tail ? listed_bits<T>(bm, min(j * NT + t0, pl.nmain) * N + BIT0) : 0u);
       }
     }
     if (ee >= 0) {
@@ -670,9 +691,11 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a
     rs.empty = __builtin_amdgcn_readfirstlane(rs.empty);
     const int slot_next = slot == 2 ? 0 : slot + 1;
     if (tid < 2) flags[grp][slot_next == 2 ? 0 : slot_next + 1][tid] = 0;  // the row before this one is through with them
-    C x_next, xy_next;
+    T x_next, xy_next;
+    const int id_next = nrow < a.nrows && tid < K ? checked(id_raw.get(a.ibits)) : -1, y_next = checked(y_raw);
     ask_scores(nrow, id_next, y_next, x_next, xy_next);
     // pass 2
+    asm volatile("" : "+s"(ap));
     const bool more = nrow < a.nrows;
     const T* xn = (const T*)a.x + (more ? nrow : row) * a.ldx;
     const Place<T> pn(xn, a.V);
@@ -680,12 +703,17 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a
     const __amdgpu_buffer_rsrc_t rg = row_rsrc(gr + pl.h, pl.nmain * 16), rn = row_rsrc(xn + pn.h, next_main * 16);
     T edge_next = (T)0.f;
     if (more && en >= 0) edge_next = xn[en];
+    int off = tid * 16;
+    opaque(off);  // NV sums that stay out of the row loop's registers
     auto entry = [&](C x, C coef) { return ex2((x - rs.M) * c) * coef + (two ? ex2((x - rs.M) * (C)LOG2E) * rs.c1 : C(0)); };
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      // (stores and loads without a branch: what lies behind a row's end is dropped by the bounds check, and the compiler can
+      // count what is in flight -- with branches here it waits for the whole row before the first vector)
+      u32x4 out;
+      opaque(d[j]);  // or the compiler keeps the unpacked vectors of pass 1, twice the registers
       if (j * NT < pl.nmain) {
         C x[N], o[N];
-        opaque(d[j]);  // or the compiler keeps the unpacked vectors of pass 1, twice the registers
         unpack<T>(d[j], x);
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i] = ex2((x[i] - rs.M) * c) * rs.cR;
@@ -693,11 +721,13 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a
 #pragma unroll
           for (int i = 0; i < N; ++i) o[i] += ex2((x[i] - rs.M) * (C)LOG2E) * rs.c1;
         }
-        stb16(rg, tid * 16 + j * NT * 16, pack<T>(o));
+        out = pack<T>(o);
       }
-      if (j * NT < next_main) d[j] = ldb16(rn, tid * 16 + j * NT * 16);
+      stb16(rg, off + j * NT * 16, out);
+      d[j] = ldb16(rn, off + j * NT * 16);
     }
     if (ee >= 0) gr[ee] = (T)entry(up<T>(edge), rs.cR);
+    asm volatile("" : "+s"(ap));
     // the list's probabilities and its part of the value; its bits go
 #pragma clang loop unroll(disable)
     for (int k = tid; k < K; k += NT) {
@@ -749,6 +779,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs a
     if (a.value != nullptr) *(C*)a.value = (C)fin[0];
   }
 }
+#undef a
 
 template <typename T, bool tail, bool two, int NT, int NV>
 pg_status run_rows(pg_ctx* c, DArgs a, int64_t rows) {
@@ -769,6 +800,7 @@ pg_status run_rows(pg_ctx* c, DArgs a, int64_t rows) {
 template <typename T, bool tail, bool two>
 pg_status run_mode(pg_ctx* c, const DArgs& a, int64_t rows) {
   const int64_t V = a.V;
+  if (a.K > 0 && !RawReal<typename Elem<T>::C>::takes(a.tdt)) return run_parts<T, tail, two>(c, a, rows);
 #define PG_ROWS_TRY(NT, NV)                                                                                                              \
   if (V <= RowsGeom<T, NT, NV>::capacity && RowsGeom<T, NT, NV>::GPW * RowsGeom<T, NT, NV>::group_bytes(a.V, a.K) <= 62 * 1024) \
   return run_rows<T, tail, two, NT, NV>(c, a, rows)
