@@ -27,7 +27,7 @@ struct BArgs {
   int64_t groups, ntiles;
   int E, k, cbits;
   double lam_e_k;  // lam * experts / k
-  double *partials, *scratch, *out;
+  double *partials, *out;
   unsigned* counter;
   void* value;
 };
@@ -256,12 +256,12 @@ __device__ __forceinline__ void zero_tile(const BArgs& a, int64_t t0, int64_t t1
 }
 
 template <typename C>
-__device__ __forceinline__ bool finish(const BArgs& a, double v_thread) {
-  double v[1] = {v_thread}, one[1] = {1.0}, fin[1];
-  const bool last = grid_reduce_finalize<1, 0, BT / 64>(v, a.partials, a.counter, a.scratch, one, fin);
-  if (last && threadIdx.x == 0) {
-    *a.out = fin[0];
-    if (a.value != nullptr) *(C*)a.value = (C)fin[0];
+__device__ __forceinline__ bool finish(const BArgs& a, double v) {
+  double total;
+  const bool last = sum_workgroups<BT / 64>(v, gridDim.x, blockIdx.x, a.partials, a.counter, total);
+  if (last) {
+    *a.out = total;
+    if (a.value != nullptr) *(C*)a.value = (C)total;
   }
   return last;
 }
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(BT) void balance_grad(BArgs a) {
     v += grad_tile<T, PL>(a, tl.begin, tl.end, sc);
     __syncthreads();
   }
-  if (finish<typename Elem<T>::C>(a, v) && threadIdx.x == 0) a.state[0] = turn ^ 1u;
+  if (finish<typename Elem<T>::C>(a, v)) a.state[0] = turn ^ 1u;
 }
 
 // both passes, a workgroup per group
@@ -406,7 +406,7 @@ extern "C" pg_status pg_balance_value_and_gradient(pg_ctx* c, const pg_balance* 
     a.tiles = b->tiles, a.mask = (const uint8_t*)b->mask, a.chosen = b->chosen, a.counts = b->counts, a.state = b->state;
     a.groups = b->groups, a.ntiles = b->ntiles, a.E = b->experts, a.k = b->k, a.cbits = b->chosen_bits;
     a.lam_e_k = b->lam * b->experts / b->k;
-    a.partials = c->red_partials, a.scratch = c->red_partials + PG_RED_MAX_BLOCKS, a.out = out, a.counter = c->red_counter, a.value = value;
+    a.partials = c->red_partials, a.out = out, a.counter = c->red_counter, a.value = value;
     const bool whole = b->whole != 0;
     if (dtype == PG_F32) PG_TRY(run<float>(c, a, whole));
     else if (dtype == PG_F64) PG_TRY(run<double>(c, a, whole));

@@ -184,9 +184,31 @@ struct Run {
 };
 
 // ---- the general form: a row in parts, two reads ------------------------------------------------------------------
-// Any length, any number of rows.  First launch: the statistics of each part (and the listed scores, which an in-place
-// gradient overwrites); second launch: every part joins its row's statistics and writes its piece of the gradient.
-constexpr int PT = 256;
+// Any length, and few rows: a part per workgroup.  First launch: the statistics of each part (and the listed scores, which an
+// in-place gradient overwrites); second launch: every part joins its row's statistics and writes its piece of the
+// gradient; the second read comes from a cache where the rows are few.  What a workgroup needs is asked for at its start.
+constexpr int PT = 256;  // threads
+constexpr int PV = 4;    // vectors of a thread at a time
+
+template <typename T>
+struct Part {
+  Place<T> pl;
+  int part, v0, v1, e0, e1, bbase, ee, words;
+  int64_t r, row;
+  __device__ __forceinline__ Part(const DArgs& a)
+      : pl((const T*)a.x + (a.row0 + blockIdx.x / a.parts) * a.ldx, a.V), part(blockIdx.x % a.parts), r(blockIdx.x / a.parts), row(a.row0 + r) {
+    constexpr int N = Elem<T>::N;
+    const int tid = threadIdx.x;
+    v0 = min(part * a.pv, pl.nmain), v1 = min(v0 + a.pv, pl.nmain);
+    const bool last = part == a.parts - 1;
+    e0 = part == 0 ? 0 : pl.h + v0 * N, e1 = last ? a.V : pl.h + v1 * N;  // its classes
+    bbase = pl.h + v0 * N - BIT0;                                         // class of bit 0
+    // thread i: the i-th element of the row's head; thread PT - 1 - i: of its tail
+    ee = part == 0 && tid < pl.h ? tid : (last && pl.hV + (PT - 1 - tid) < a.V ? pl.hV + (PT - 1 - tid) : -1);
+    words = (a.pv * N + BIT0 + N + 31) / 32;
+  }
+  __device__ __forceinline__ bool has(int64_t e) const { return e >= e0 && e < e1; }
+};
 
 template <typename T, bool TAIL, bool TWO>
 __global__ __launch_bounds__(PT) void distill_part_stats(DArgs a) {
@@ -195,52 +217,54 @@ __global__ __launch_bounds__(PT) void distill_part_stats(DArgs a) {
   extern __shared__ unsigned bm[];
   __shared__ C sm[PT / 64][5];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int part = blockIdx.x % a.parts;
-  const int64_t r = blockIdx.x / a.parts, row = a.row0 + r;
-  if (a.w != nullptr && ld_real(a.w, a.wdt, row) == 0.0) return;
-  const T* xr = (const T*)a.x + row * a.ldx;
-  const Place<T> pl(xr, a.V);
-  const int v0 = min(part * a.pv, pl.nmain), v1 = min(v0 + a.pv, pl.nmain);
-  const bool lastp = part == a.parts - 1;
-  const int e0 = part == 0 ? 0 : pl.h + v0 * N, e1 = lastp ? a.V : pl.h + v1 * N;
-  const int bbase = pl.h + v0 * N - BIT0;  // element of bit 0
-  const int words = (a.pv * N + BIT0 + N + 31) / 32;
+  const Part<T> q(a);
+  if (a.w != nullptr && ld_real_u(a.w, a.wdt, q.row) == 0.0) return;
+  const T* xr = (const T*)a.x + q.row * a.ldx;
+  const T* xm = xr + q.pl.h;
+  u32x4 d[PV];
+  auto load = [&](int v) {
+#pragma unroll
+    for (int j = 0; j < PV; ++j) d[j] = v + j * PT < q.v1 ? ld16(at16(xm, v + j * PT)) : minus_inf16<T>();
+  };
+  load(q.v0 + tid);
+  const T edge = q.ee >= 0 ? xr[q.ee] : (T)0.f;
   if constexpr (TAIL) {
-    for (int i = tid; i < words; i += PT) bm[i] = 0;
+    for (int i = tid; i < q.words; i += PT) bm[i] = 0;
     __syncthreads();
   }
   Run<C, TAIL, TWO> run(a.invT);
   bool bad = false;
   for (int k = tid; k < a.K; k += PT) {
-    const int64_t id = ld_int(a.idx, a.ibits, row * a.ldi + k);
+    const int64_t id = ld_int(a.idx, a.ibits, q.row * a.ldi + k);
     bad |= id < -1 || id >= a.V;
-    if (id >= e0 && id < e1) {
+    if (q.has(id)) {
       const C x = up<T>(xr[id]);
-      a.xk[r * (a.K + 1) + k] = (double)x;
+      a.xk[q.r * (a.K + 1) + k] = (double)x;
       if constexpr (TAIL) {
-        const int b = (int)id - bbase;
+        const int b = (int)id - q.bbase;
         const unsigned old = atomicOr(&bm[b >> 5], 1u << (b & 31));
         if (!((old >> (b & 31)) & 1u)) run.listed(x);
       }
     }
   }
   if (tid == 0 && a.lab != nullptr) {
-    const int64_t y = ld_int(a.lab, a.labbits, row);
+    const int64_t y = ld_int_u(a.lab, a.labbits, q.row);
     bad |= y < -1 || y >= a.V;
-    if (y >= e0 && y < e1) a.xk[r * (a.K + 1) + a.K] = (double)up<T>(xr[y]);
+    if (q.has(y)) a.xk[q.r * (a.K + 1) + a.K] = (double)up<T>(xr[y]);
   }
   if constexpr (TAIL) __syncthreads();
-  const T* xm = xr + pl.h;
-  for (int v = v0 + tid; v < v1; v += PT) {
-    C f[N];
-    unpack<T>(ld16(at16(xm, v)), f);
-    run.template add<N>(f, TAIL ? listed_bits<T>(bm, (v - v0) * N + BIT0) : 0u);
+  for (int v = q.v0 + tid; v - tid < q.v1; v += PV * PT) {
+    if (v != q.v0 + tid) load(v);
+#pragma unroll
+    for (int j = 0; j < PV; ++j) {
+      C f[N];
+      unpack<T>(d[j], f);
+      run.template add<N>(f, TAIL ? listed_bits<T>(bm, min(v + j * PT - q.v0, q.v1 - q.v0) * N + BIT0) : 0u);
+    }
   }
-  // (thread i: the i-th element of the head; thread PT - 1 - i: of the tail)
-  const int ee = part == 0 && tid < pl.h ? tid : (lastp && pl.hV + (PT - 1 - tid) < a.V ? pl.hV + (PT - 1 - tid) : -1);
-  if (ee >= 0) {
-    const int b = ee - bbase;
-    run.add1(up<T>(xr[ee]), TAIL && ((bm[b >> 5] >> (b & 31)) & 1u));
+  if (q.ee >= 0) {
+    const int b = q.ee - q.bbase;
+    run.add1(up<T>(edge), TAIL && ((bm[b >> 5] >> (b & 31)) & 1u));
   }
   if (bad) run.s = (C)NAN;
   const C M = wave_max(run.m);
@@ -260,7 +284,7 @@ __global__ __launch_bounds__(PT) void distill_part_stats(DArgs a) {
       if constexpr (TWO) o[2] += sm[i][3] * ex2((sm[i][0] - m) * (C)LOG2E);
       o[3] += sm[i][4];
     }
-    double* st = a.stat + (r * a.parts + part) * STAT;
+    double* st = a.stat + (q.r * a.parts + q.part) * STAT;
     st[0] = (double)m;
     for (int i = 0; i < 4; ++i) st[1 + i] = (double)o[i];
   }
@@ -271,123 +295,144 @@ __global__ __launch_bounds__(PT) void distill_part_grad(DArgs a) {
   using C = typename Elem<T>::C;
   constexpr int N = Elem<T>::N;
   extern __shared__ unsigned bm[];
-  __shared__ double smd[PT / 64][2];
+  __shared__ C smt[PT / 64][2];
+  __shared__ double smd[PT / 64];
   __shared__ int dup;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int part = blockIdx.x % a.parts;
-  const int64_t r = blockIdx.x / a.parts, row = a.row0 + r;
-  const T* xr = (const T*)a.x + row * a.ldx;
-  T* gr = (T*)a.g + row * a.ldg;
-  const Place<T> pl(xr, a.V);
-  const int v0 = min(part * a.pv, pl.nmain), v1 = min(v0 + a.pv, pl.nmain);
-  const bool lastp = part == a.parts - 1;
-  const int e0 = part == 0 ? 0 : pl.h + v0 * N, e1 = lastp ? a.V : pl.h + v1 * N;
-  const int bbase = pl.h + v0 * N - BIT0;
-  const int ee = part == 0 && tid < pl.h ? tid : (lastp && pl.hV + (PT - 1 - tid) < a.V ? pl.hV + (PT - 1 - tid) : -1);
-  const double w = a.w != nullptr ? ld_real(a.w, a.wdt, row) : 1.0;
+  const Part<T> q(a);
+  const T* xr = (const T*)a.x + q.row * a.ldx;
+  const T* xm = xr + q.pl.h;
+  T* gr = (T*)a.g + q.row * a.ldg;
+  T* gm = gr + q.pl.h;
+  const double w = a.w != nullptr ? ld_real_u(a.w, a.wdt, q.row) : 1.0;
   double v_row = 0.0;
   if (w == 0.0) {
     const u32x4 zero = {0u, 0u, 0u, 0u};
-    for (int v = v0 + tid; v < v1; v += PT) st16(at16(gr + pl.h, v), zero);
-    if (ee >= 0) gr[ee] = (T)0.f;
+    for (int v = q.v0 + tid; v < q.v1; v += PT) st16(at16(gm, v), zero);
+    if (q.ee >= 0) gr[q.ee] = (T)0.f;
   } else {
-    const int words = (a.pv * N + BIT0 + N + 31) / 32;
-    for (int i = tid; i < words; i += PT) bm[i] = 0;
+    u32x4 d[PV];
+    auto load = [&](int v) {
+#pragma unroll
+      for (int j = 0; j < PV; ++j) d[j] = v + j * PT < q.v1 ? ld16(at16(xm, v + j * PT)) : minus_inf16<T>();
+    };
+    // the row's parts, one lane each
+    const double* st = a.stat + q.r * a.parts * STAT;
+    const int mine = min(lane, a.parts - 1) * STAT;
+    const C pm = (C)st[mine], ps = (C)st[mine + 1], pl = TAIL ? (C)st[mine + 2] : C(0), p1 = TWO ? (C)st[mine + 3] : C(0),
+            pn = TAIL ? (C)st[mine + 4] : C(0);
+    load(q.v0 + tid);
+    const T edge = q.ee >= 0 ? xr[q.ee] : (T)0.f;
+    for (int i = tid; i < q.words; i += PT) bm[i] = 0;
     if (tid == 0) dup = 0;
     __syncthreads();
-    const int64_t y = a.lab != nullptr ? ld_int(a.lab, a.labbits, row) : -1;
+    const int64_t y = a.lab != nullptr ? ld_int_u(a.lab, a.labbits, q.row) : -1;
+    const double lse = TAIL ? ld_real_u(a.lse, a.lsedt, q.row) : 0.0;
     // the teacher's side: log normaliser and listed mass
-    double tm = -INFINITY, ts = 0.0;
+    C tm = Lim<C>::lowest, ts = C(0);
+    double tmass = 0.0;
     for (int k = tid; k < a.K; k += PT) {
-      const int64_t id = ld_int(a.idx, a.ibits, row * a.ldi + k);
+      const int64_t id = ld_int(a.idx, a.ibits, q.row * a.ldi + k);
       if (id < 0 || id >= a.V) continue;
-      if (id >= e0 && id < e1) {
-        const int b = (int)id - bbase;
+      if (q.has(id)) {
+        const int b = (int)id - q.bbase;
         if ((atomicOr(&bm[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1u) dup = 1;
       }
-      const double t = ld_real(a.t, a.tdt, row * a.ldt + k) * a.invT;
+      const double t = ld_real(a.t, a.tdt, q.row * a.ldt + k) * a.invT;
       if constexpr (TAIL) {
-        ts += exp(t - ld_real(a.lse, a.lsedt, row));
-      } else if (t > tm || t != t) {
-        ts = t != t ? t : ts * exp(tm - t) + 1.0;
-        if (t > tm) tm = t;
-      } else if (t > -INFINITY) {
-        ts += exp(t - tm);
+        tmass += exp_series(t - lse);
+      } else {
+        const C tc = (C)t;
+        if (tc > tm) {
+          ts *= ex2((tm - tc) * (C)LOG2E);
+          tm = tc;
+        }
+        ts += ex2((tc - tm) * (C)LOG2E);
       }
     }
-    const double wm = wave_max(tm);
-    const double wsum = wave_sum(TAIL || tm == -INFINITY ? ts : ts * exp(tm - wm));
-    if (lane == 0) smd[wave][0] = wm, smd[wave][1] = wsum;
+    if constexpr (TAIL) {
+      tmass = wave_sum(tmass);
+      if (lane == 0) smd[wave] = tmass;
+    } else {
+      const C wm = wave_max(tm);
+      ts = wave_sum(ts * ex2((tm - wm) * (C)LOG2E));
+      if (lane == 0) smt[wave][0] = wm, smt[wave][1] = ts;
+    }
     __syncthreads();
-    tm = smd[0][0];
-    for (int i = 1; i < PT / 64; ++i) tm = fmax(tm, smd[i][0]);
-    ts = 0.0;
-    for (int i = 0; i < PT / 64; ++i) ts += TAIL || smd[i][0] == -INFINITY ? smd[i][1] : smd[i][1] * exp(smd[i][0] - tm);
-    const double norm = TAIL ? ld_real(a.lse, a.lsedt, row) : tm + log(ts);
-    const double mass = TAIL ? ts : (ts == 0.0 ? 0.0 : ts / ts);  // a list without mass: no teacher
-    // the row's parts joined, one lane each
-    const double* st = a.stat + r * a.parts * STAT;
+    double norm, mass;
+    if constexpr (TAIL) {
+      norm = lse;
+      mass = smd[0];
+      for (int i = 1; i < PT / 64; ++i) mass += smd[i];
+    } else {
+      tm = smt[0][0];
+      for (int i = 1; i < PT / 64; ++i) tm = fmx(tm, smt[i][0]);
+      ts = C(0);
+      for (int i = 0; i < PT / 64; ++i) ts += smt[i][1] * ex2((smt[i][0] - tm) * (C)LOG2E);
+      norm = (double)tm + (double)(lg2(ts) * (C)LN2);
+      mass = ts == C(0) ? 0.0 : (double)(ts / ts);  // a list without mass: no teacher
+    }
     const bool in = lane < a.parts;
-    const C pm = in ? (C)st[lane * STAT] : Lim<C>::lowest;
     const C M = wave_max(pm);
     const C c = (C)(a.invT * LOG2E);
     const C f = ex2((pm - M) * c);
-    const C s = wave_sum(in ? (C)st[lane * STAT + 1] * f : C(0));
-    const C sl = TAIL ? wave_sum(in ? (C)st[lane * STAT + 2] * f : C(0)) : C(0);
-    const C s1 = TWO ? wave_sum(in ? (C)st[lane * STAT + 3] * ex2((pm - M) * (C)LOG2E) : C(0)) : C(0);
-    const C nl = TAIL ? wave_sum(in ? (C)st[lane * STAT + 4] : C(0)) : C(0);
+    const C s = wave_sum(in ? ps * f : C(0)), sl = TAIL ? wave_sum(in ? pl * f : C(0)) : C(0), nl = TAIL ? wave_sum(in ? pn : C(0)) : C(0);
+    const C s1 = TWO ? wave_sum(in ? p1 * ex2((pm - M) * (C)LOG2E) : C(0)) : C(0);
     const RowScal<C> rs = row_scalars<C>(a, TAIL, TWO, w, y >= 0, M, s, sl, s1, nl, mass);
-    for (int v = v0 + tid; v < v1; v += PT) {
-      C x[N], o[N];
-      unpack<T>(ld16(at16(xr + pl.h, v)), x);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        o[i] = ex2((x[i] - rs.M) * c) * rs.cR;
-        if constexpr (TWO) o[i] += ex2((x[i] - rs.M) * (C)LOG2E) * rs.c1;
-      }
-      st16(at16(gr + pl.h, v), pack<T>(o));
-    }
     auto entry = [&](C x, C coef) { return ex2((x - rs.M) * c) * coef + (TWO ? ex2((x - rs.M) * (C)LOG2E) * rs.c1 : C(0)); };
-    if (ee >= 0) gr[ee] = (T)entry(up<T>(xr[ee]), rs.cR);
+    for (int v = q.v0 + tid; v - tid < q.v1; v += PV * PT) {
+      if (v != q.v0 + tid) load(v);
+#pragma unroll
+      for (int j = 0; j < PV; ++j) {
+        if (v + j * PT >= q.v1) continue;
+        C x[N], o[N];
+        unpack<T>(d[j], x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = entry(x[i], rs.cR);
+        st16(at16(gm, v + j * PT), pack<T>(o));
+      }
+    }
+    if (q.ee >= 0) gr[q.ee] = (T)entry(up<T>(edge), rs.cR);
     __syncthreads();  // the vectors are written: the listed entries go over them
-    const double* xk = a.xk + r * (a.K + 1);
+    const double* xk = a.xk + q.r * (a.K + 1);
     for (int k = tid; k < a.K; k += PT) {
-      const int64_t id = ld_int(a.idx, a.ibits, row * a.ldi + k);
+      const int64_t id = ld_int(a.idx, a.ibits, q.row * a.ldi + k);
       if (id < 0 || id >= a.V) continue;
       C lp, p;
-      entry_p<C>(a, row, k, norm, lp, p);
+      entry_p<C>(a, q.row, k, norm, lp, p);
       const C x = (C)xk[k];
-      if (part == 0 && !rs.empty && p != C(0)) v_row += a.lam * w * (double)(p * (lp - ((x - rs.M) * (C)a.invT - rs.ls)));
-      if (id >= e0 && id < e1) {
+      if (q.part == 0 && !rs.empty && p != C(0)) v_row += a.lam * w * (double)(p * (lp - ((x - rs.M) * (C)a.invT - rs.ls)));
+      if (q.has(id)) {
         C ph = p;
         bool owner = true;
         if (dup) {  // a class listed twice: its first entry writes the sum
-          for (int q = 0; q < a.K; ++q) {
-            if (q == k || ld_int(a.idx, a.ibits, row * a.ldi + q) != id) continue;
-            owner &= q > k;
-            C lq, pq;
-            entry_p<C>(a, row, q, norm, lq, pq);
-            ph += pq;
+          for (int o = 0; o < a.K; ++o) {
+            if (o == k || ld_int(a.idx, a.ibits, q.row * a.ldi + o) != id) continue;
+            owner &= o > k;
+            C lo, po;
+            entry_p<C>(a, q.row, o, norm, lo, po);
+            ph += po;
           }
         }
         if (owner) gr[id] = (T)(entry(x, rs.cB) - rs.ql * ph - (id == y ? rs.qy : C(0)));
       }
     }
     if (tid == PT - 1) {
-      if (y >= e0 && y < e1) {
-        const int b = (int)y - bbase;
+      if (q.has(y)) {
+        const int b = (int)y - q.bbase;
         if (!((bm[b >> 5] >> (b & 31)) & 1u)) gr[y] = (T)(entry((C)xk[a.K], rs.cR) - rs.qy);
       }
-      if (part == 0 && !rs.empty) {
+      if (q.part == 0 && !rs.empty) {
         if (TAIL && rs.pr != 0.0) v_row += a.lam * w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - rs.log_qr);
         if (y >= 0 && y < a.V) v_row += a.lab_lam * w * (double)(rs.ls1 - ((C)xk[a.K] - rs.M));
-        if (rs.ls != rs.ls) v_row = NAN;  // a NaN score, or an index or label out of range
       }
+      if (rs.ls != rs.ls) v_row = NAN;  // a NaN score, or an index or label out of range
     }
   }
-  double v[1] = {v_row}, one[1] = {1.0}, fin[1];
-  if (grid_reduce_finalize<1, 0, PT / 64>(v, a.partials, a.counter, a.acc + 1, one, fin) && threadIdx.x == 0) {
-    const double total = a.first ? fin[0] : *a.acc + fin[0];
+  if (q.part != 0) return;  // the first part of each row carries its value
+  double total;
+  if (sum_workgroups<PT / 64>(v_row, (unsigned)a.nrows, (unsigned)q.r, a.partials, a.counter, total)) {
+    if (!a.first) total += *a.acc;
     *a.acc = total;
     if (a.last) {
       *a.out = total;
@@ -400,21 +445,21 @@ template <typename T, bool TAIL, bool TWO>
 pg_status run_parts(pg_ctx* c, DArgs a, int64_t rows) {
   constexpr int N = Elem<T>::N;
   const int64_t vecs = (a.V + N - 1) / N;
-  // a part: at least 1024 vectors (16 KiB), at most what the bitmap holds; enough parts for two workgroups per CU
+  // two workgroups per CU if the rows are few, but no part below 2 vectors a thread, and none that its bitmap does not hold
   const int64_t most = (32 * 1024 * 8) / N;
   int64_t parts = (2 * c->num_cu + rows - 1) / rows;
-  parts = std::min<int64_t>(parts, (vecs + 1023) / 1024);
+  parts = std::min<int64_t>(parts, (vecs + 2 * PT - 1) / (2 * PT));
   parts = std::max<int64_t>(parts, (vecs + most - 1) / most);
   parts = std::max<int64_t>(1, std::min<int64_t>(parts, MAX_PARTS));
   a.parts = (int)parts;
   a.pv = (int)((vecs + parts - 1) / parts);
   const size_t lds = ((size_t)a.pv * N + BIT0 + N + 31) / 32 * 4 + 4;
-  if (lds > 64 * 1024) {
-    pg_set_error("pg_distill: rows of more than %lld classes are not supported for this type", (long long)(64 * 1024 * 8 / N * N) * MAX_PARTS);
+  if (lds > 62 * 1024) {
+    pg_set_error("pg_distill: rows of more than %lld classes are not supported", (long long)MAX_PARTS * 62 * 1024 * 8);
     return PG_ERR_UNSUPPORTED;
   }
   const int64_t ws = (int64_t)PG_RED_MAX_BLOCKS * (PG_RED_MAX_NS - 1) - 8;  // doubles behind the reduction's own partials
-  int64_t batch = std::min<int64_t>(ws / (parts * STAT + a.K + 1), PG_RED_MAX_BLOCKS / parts);
+  const int64_t batch = std::min<int64_t>(ws / (parts * STAT + a.K + 1), PG_RED_MAX_BLOCKS);
   a.acc = c->red_partials + PG_RED_MAX_BLOCKS;
   a.stat = a.acc + 8;
   for (int64_t r0 = 0; r0 < rows; r0 += batch) {
@@ -431,7 +476,6 @@ pg_status run_parts(pg_ctx* c, DArgs a, int64_t rows) {
   }
   return PG_OK;
 }
-
 
 // ---- the row in registers: one read, one write ---------------------------------------------------------------------
 // NT threads hold a row as NV 16-byte vectors each (NT = 64: a wave per row, four rows per workgroup; else a workgroup per row).
@@ -773,10 +817,10 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     par ^= 1;
     slot = slot_next;
   }
-  double v[1] = {v_acc}, one[1] = {1.0}, fin[1];
-  if (grid_reduce_finalize<1, 0, G::WG / 64>(v, a.partials, a.counter, a.acc + 1, one, fin) && threadIdx.x == 0) {
-    *a.out = fin[0];
-    if (a.value != nullptr) *(C*)a.value = (C)fin[0];
+  double total;
+  if (sum_workgroups<G::WG / 64>(v_acc, gridDim.x, blockIdx.x, ap->partials, ap->counter, total)) {
+    *ap->out = total;
+    if (ap->value != nullptr) *(C*)ap->value = (C)total;
   }
 }
 #undef a
@@ -787,11 +831,14 @@ pg_status run_rows(pg_ctx* c, DArgs a, int64_t rows) {
   const size_t lds = (size_t)G::group_bytes(a.V, a.K) * G::GPW;
   a.acc = c->red_partials + PG_RED_MAX_BLOCKS;
   a.nrows = rows;
-  int per_cu = 0;
   void (*kernel)(DArgs) = distill_rows<T, NT, NV, tail, two>;
-  PG_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, G::WG, lds));
+  static const int by_registers = [&] {
+    int n = 0;
+    return hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, G::WG, 0) == hipSuccess ? std::max(n, 1) : 1;
+  }();
+  const int per_cu = std::min(by_registers, std::max(1, (int)(160 * 1024 / (lds + 1024))));
   const int64_t want = (rows + G::GPW - 1) / G::GPW;
-  const int64_t grid = std::min<int64_t>(std::min<int64_t>(want, PG_RED_MAX_BLOCKS), (int64_t)std::max(per_cu, 1) * c->num_cu);
+  const int64_t grid = std::min<int64_t>(std::min<int64_t>(want, PG_RED_MAX_BLOCKS), (int64_t)per_cu * c->num_cu);
   kernel<<<(unsigned)grid, G::WG, lds, c->stream>>>(a);
   PG_LAUNCH_CHECK();
   return PG_OK;

@@ -70,6 +70,13 @@ def _common_device(tensors, ctx):
     return ctx
 
 
+def _raw_stream(device):
+    """the current torch stream's handle (every call looks: torch's own accessor makes a Stream object each time)"""
+    torch = _torch()
+    fast = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return fast(device) if fast is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 class _Ordered:
     """the call's kernels run on the context's stream: between the current torch stream's past and its future"""
 
@@ -84,8 +91,8 @@ class _Ordered:
         self.cur = None
         if ctx.capturing:
             return
-        cur = torch.cuda.current_stream(ctx.torch_device)
-        if cur.cuda_stream != ctx.stream:
+        if _raw_stream(ctx.device) != ctx.stream:
+            cur = torch.cuda.current_stream(ctx.torch_device)
             with torch.cuda.device(ctx.device):
                 if torch.cuda.is_current_stream_capturing():
                     raise ProxGradError("a torch graph is being recorded: record with Context.capture_begin instead",
