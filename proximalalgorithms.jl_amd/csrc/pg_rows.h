@@ -273,6 +273,10 @@ __device__ __forceinline__ bool sum_workgroups(double v, unsigned n, unsigned me
     return t;
   };
   const double mine = join(v);
+  if (n == 1) {
+    total = mine;
+    return threadIdx.x == 0;
+  }
   if (threadIdx.x == 0) {
     __hip_atomic_store(&partials[me], mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -285,6 +289,13 @@ __device__ __forceinline__ bool sum_workgroups(double v, unsigned n, unsigned me
   total = join(acc);
   if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   return threadIdx.x == 0;
+}
+
+// the value where it was asked for: the context's scalar block (host memory) and the caller's device scalar
+template <typename C>
+__device__ __forceinline__ void store_value(double v, double* out, void* value) {
+  if (out != nullptr) *out = v;
+  if (value != nullptr) *(C*)value = (C)v;
 }
 
 // NT threads of one workgroup work on a row: all of it (a workgroup's barrier) or one wave of it (its LDS accesses are in order)

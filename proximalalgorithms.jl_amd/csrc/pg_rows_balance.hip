@@ -260,8 +260,7 @@ __device__ __forceinline__ bool finish(const BArgs& a, double v) {
   double total;
   const bool last = sum_workgroups<BT / 64>(v, gridDim.x, blockIdx.x, a.partials, a.counter, total);
   if (last) {
-    *a.out = total;
-    if (a.value != nullptr) *(C*)a.value = (C)total;
+    store_value<C>(total, a.out, a.value);
   }
   return last;
 }
@@ -364,11 +363,8 @@ pg_status run(pg_ctx* c, const BArgs& a, bool whole) {
 }
 
 __global__ void balance_zero(double* out, void* value, int f64) {
-  *out = 0.0;
-  if (value != nullptr) {
-    if (f64) *(double*)value = 0.0;
-    else *(float*)value = 0.f;
-  }
+  if (f64) store_value<double>(0.0, out, value);
+  else store_value<float>(0.0, out, value);
 }
 
 }  // namespace
@@ -396,7 +392,7 @@ extern "C" pg_status pg_balance_value_and_gradient(pg_ctx* c, const pg_balance* 
   DeviceScope dev(c->device);
   PG_TRY(dev.st);
   PG_TRY(refuse_foreign_capture(c));
-  double* out = c->dscal + PG_S_MISC;
+  double* out = f_out != nullptr ? c->dscal + PG_S_MISC : nullptr;
   if (!any) {
     balance_zero<<<1, 1, 0, c->stream>>>(out, value, dtype == PG_F64);
     PG_LAUNCH_CHECK();

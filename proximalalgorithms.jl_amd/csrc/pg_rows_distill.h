@@ -434,10 +434,7 @@ __global__ __launch_bounds__(PT) void distill_part_grad(DArgs a) {
   if (sum_workgroups<PT / 64>(v_row, (unsigned)a.nrows, (unsigned)q.r, a.partials, a.counter, total)) {
     if (!a.first) total += *a.acc;
     *a.acc = total;
-    if (a.last) {
-      *a.out = total;
-      if (a.value != nullptr) *(C*)a.value = (C)total;
-    }
+    if (a.last) store_value<C>(total, a.out, a.value);
   }
 }
 
@@ -819,8 +816,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
   }
   double total;
   if (sum_workgroups<G::WG / 64>(v_acc, gridDim.x, blockIdx.x, ap->partials, ap->counter, total)) {
-    *ap->out = total;
-    if (ap->value != nullptr) *(C*)ap->value = (C)total;
+    store_value<C>(total, ap->out, ap->value);
   }
 }
 #undef a
@@ -847,6 +843,10 @@ pg_status run_rows(pg_ctx* c, DArgs a, int64_t rows) {
 template <typename T, bool tail, bool two>
 pg_status run_mode(pg_ctx* c, const DArgs& a, int64_t rows) {
   const int64_t V = a.V;
+  // Few long rows: a workgroup each leaves most of the device idle and takes 11 us for 64 KiB, 19 us for 256 KiB however few they
+  // are; in parts 9 us.  At 64 rows of 64 / 256 KiB 10.7 / 16.1 us against 12.7 / 22.2, at 128 rows 11.9 / 24.7 against
+  // 13.1 / 23.7, and below 64 KiB a row one launch is the faster at any number (bf16; Float32 of the same bytes alike).
+  if (rows <= c->num_cu / 4 && V >= 4096 * Elem<T>::N) return run_parts<T, tail, two>(c, a, rows);
   if (a.K > 0 && !RawReal<typename Elem<T>::C>::takes(a.tdt)) return run_parts<T, tail, two>(c, a, rows);
 #define PG_ROWS_TRY(NT, NV)                                                                                                              \
   if (V <= RowsGeom<T, NT, NV>::capacity && RowsGeom<T, NT, NV>::GPW * RowsGeom<T, NT, NV>::group_bytes(a.V, a.K) <= 62 * 1024) \

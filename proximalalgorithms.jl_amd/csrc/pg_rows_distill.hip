@@ -4,11 +4,8 @@
 namespace pgrows {
 namespace {
 __global__ void store_zero(double* out, void* value, int f64) {
-  *out = 0.0;
-  if (value != nullptr) {
-    if (f64) *(double*)value = 0.0;
-    else *(float*)value = 0.f;
-  }
+  if (f64) store_value<double>(0.0, out, value);
+  else store_value<float>(0.0, out, value);
 }
 
 }  // namespace
@@ -46,7 +43,7 @@ pg_status pg_distill_value_and_gradient(pg_ctx* c, const pg_distill* d, int32_t 
   DeviceScope dev(c->device);
   PG_TRY(dev.st);
   PG_TRY(refuse_foreign_capture(c));
-  double* out = c->dscal + PG_S_MISC;
+  double* out = f_out != nullptr ? c->dscal + PG_S_MISC : nullptr;
   if (!any) {
     store_zero<<<1, 1, 0, c->stream>>>(out, value, dtype == PG_F64);
     PG_LAUNCH_CHECK();

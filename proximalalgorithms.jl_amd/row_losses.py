@@ -14,23 +14,26 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import PG_BF16, PG_F16, PG_F32, PG_F64, ProxGradError, call
+from ._lib import PG_BF16, PG_F16, PG_F32, PG_F64, ProxGradError
 from .device import HIPVector, get_context
 
 
-def _torch():
-    import torch
-
-    return torch
-
-
+_torch_module = None
 _DTYPES = {}
 
 
-def _dtype_code(dt):
-    if not _DTYPES:
-        torch = _torch()
+def _torch():
+    global _torch_module
+    if _torch_module is None:
+        import torch
+
         _DTYPES.update({torch.float32: PG_F32, torch.float64: PG_F64, torch.bfloat16: PG_BF16, torch.float16: PG_F16})
+        _torch_module = torch
+    return _torch_module
+
+
+def _dtype_code(dt):
+    _torch()
     return _DTYPES.get(dt)
 
 
@@ -123,18 +126,21 @@ class _RowLoss:
         code = _dtype_code(getattr(u, "dtype", None))
         if code is None:
             raise TypeError(f"{name} must be a HIPVector or a Float32, Float64, bfloat16 or Float16 torch tensor")
-        if not u.is_cuda or u.device.index != self.ctx.device:
+        if u.get_device() != self.ctx.device:  # -1 on the host
             raise ValueError(f"{name} must live on the loss's device {self.ctx.device}")
-        if tuple(u.shape) != (n, v) and not (u.dim() == 1 and u.shape[0] == n * v and (n * v == 0 or u.stride(0) == 1)):
-            raise ValueError(f"{name} must have shape ({n}, {v}), got {tuple(u.shape)}")
-        if u.dim() == 1:
+        shape = u.shape
+        if len(shape) == 2 and shape[0] == n and shape[1] == v:
+            ld, step = u.stride()
+            if v > 1 and step != 1:
+                raise ValueError(f"the scores of a row of {name} must be adjacent (stride 1)")
+            if n <= 1:
+                ld = max(v, 1)
+            elif ld < v:
+                raise ValueError(f"the rows of {name} overlap")
+            return u.data_ptr(), ld, code
+        if len(shape) == 1 and shape[0] == n * v and (n * v == 0 or u.stride(0) == 1):
             return u.data_ptr(), max(v, 1), code
-        if v > 1 and u.stride(1) != 1:
-            raise ValueError(f"the scores of a row of {name} must be adjacent (stride 1)")
-        ld = u.stride(0) if n > 1 else max(v, 1)
-        if ld < v:
-            raise ValueError(f"the rows of {name} overlap")
-        return u.data_ptr(), ld, code
+        raise ValueError(f"{name} must have shape ({n}, {v}), got {tuple(shape)}")
 
     def _like(self, u):
         if isinstance(u, HIPVector):
@@ -179,8 +185,11 @@ class _RowLoss:
             value = torch.empty((), dtype=vdt, device=self.ctx.torch_device)
         elif value.numel() != 1 or value.dtype != vdt or not value.is_cuda or value.device.index != self.ctx.device:
             raise ValueError(f"value must be a one-element {vdt} tensor on the loss's device")
-        with _Ordered(self.ctx):
+        if _raw_stream(self.ctx.device) == self.ctx.stream:
             self._evaluate(where, value.data_ptr(), None)
+        else:
+            with _Ordered(self.ctx):
+                self._evaluate(where, value.data_ptr(), None)
         return value, out
 
     def __call__(self, u):
@@ -247,10 +256,13 @@ class DistillationLoss(_RowLoss):
                                   weights_dtype=code(weights), label_bits=bits(labels), temperature=self.temperature, lam=self.lam,
                                   label_lam=self.label_lam)
         self._dref = C.byref(self._d)
+        self._entry = _lib.load().pg_distill_value_and_gradient
 
     def _evaluate(self, where, value, f_out):
         up, uld, op, old, code = where
-        call("pg_distill_value_and_gradient", self.ctx.handle, self._dref, code, up, uld, op, old, value, f_out)
+        status = self._entry(self.ctx.handle, self._dref, code, up, uld, op, old, value, f_out)
+        if status:
+            _lib.check(status)
 
 
 def _balance_tiles(tokens, offsets, num_cu):
@@ -333,6 +345,7 @@ class BalanceLoss(_RowLoss):
                                   state=ptr(state), experts=self.classes, k=self.k,
                                   chosen_bits=64 if chosen is not None and chosen.dtype == torch.int64 else 32, whole=whole, lam=self.lam)
         self._bref = C.byref(self._b)
+        self._entry = _lib.load().pg_balance_value_and_gradient
 
     @property
     def counts(self):
@@ -340,4 +353,6 @@ class BalanceLoss(_RowLoss):
 
     def _evaluate(self, where, value, f_out):
         up, uld, op, old, code = where
-        call("pg_balance_value_and_gradient", self.ctx.handle, self._bref, code, up, uld, op, old, value, f_out)
+        status = self._entry(self.ctx.handle, self._bref, code, up, uld, op, old, value, f_out)
+        if status:
+            _lib.check(status)
