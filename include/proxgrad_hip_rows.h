@@ -69,14 +69,14 @@ pg_status pg_distill_value_and_gradient(pg_ctx* ctx, const pg_distill* d, int32_
  *   df/dr_tj = a_g p_tj (c_gj - sum_e c_ge p_te),  a_g = lam experts / (k n_g^2)      (the counts held fixed)
  * chosen == NULL: a token chooses its k highest scores, the lowest index first among equal ones; -inf and NaN are never chosen.
  * chosen: the router's own choices [tokens x k], -1 = none; an expert named twice counts twice.
- * A masked token is not read (its choices neither), its gradient is zero.  A token whose scores are all -inf has gradient zero.
+ * A masked token counts for nothing, whatever its scores and choices hold, and its gradient is zero.  A token whose scores are all -inf has gradient zero.
  * A NaN among a token's scores makes f and that token's gradient NaN; a choice outside [-1, experts) makes f and its
  * group's gradients NaN.  A group without unmasked tokens contributes nothing.  The tiles say what is read and written:
  * tokens of a tile of group -1 belong to no group and get a zero gradient, tokens of no tile are left alone. */
 typedef struct pg_balance_tile {
   int64_t begin, end; /* tokens [begin, end) of one group */
   int32_t group;      /* -1: tokens of no group */
-  int32_t part; /* 0: the group's first tile; -1: the group's only tile */
+  int32_t part; /* its number within the group; -1: the group's only tile */
 } pg_balance_tile;
 typedef struct pg_balance {
   int64_t tokens, groups, ntiles; /* tokens < 2^31 */
@@ -85,9 +85,10 @@ typedef struct pg_balance {
   const void* chosen;             /* [tokens x k] int32 or int64; NULL: the k highest */
   int64_t chosen_ld;
   int32_t* counts;  /* device [groups x experts]: c of the last evaluation (groups without tiles are left alone) */
-  uint32_t* state;  /* device, 4 + 2 * groups * (experts + 2) words, zero before the first evaluation: this loss's own */
+  uint32_t* state;  /* device, 4 + 2 * groups * copies * (experts + 2) words, zero before the first evaluation: this loss's own */
   int32_t experts, k, chosen_bits; /* 1 <= k <= experts <= 1024 */
-  int32_t whole;                   /* every tile is a whole group: one launch */
+  int32_t whole;                   /* every tile is a whole group: one launch (state: 4 words) */
+  int32_t copies, reserved;        /* accumulators per group that its tiles take in turn, >= 1 */
   double lam;
 } pg_balance;
 

@@ -5,9 +5,11 @@
 // counts -- integers, so that atomics give the same result in any order, and no exponentials.  Where a group is one
 // tile, a workgroup does both passes and the second one finds the scores in the cache.
 //
-// One wave takes a token, lane l its experts l * PL .. l * PL + PL - 1, so that lane order is index order.  The k-th highest
-// score is found by bisection over the scores' bit patterns (mapped to unsigned numbers in the scores' order): a step is PL
-// compares whose 64-bit masks are counted in scalar registers, whatever k is, and starts from the previous token's threshold.
+// L lanes take a token, 64 / L tokens a wave: lane l of them holds, in chunk i, the V experts from (i L + l) V on (16 bytes, so that a
+// token's chunk is read in one piece).  The k-th highest score is found by bisection over the scores' bit patterns, mapped to
+// unsigned numbers in the scores' order: a step counts the keys from a threshold on, whatever k is, all tokens of the wave
+// at once, and starts from the thresholds of the wave's tokens before.  (With a token per wave the search runs in scalar
+// registers, on the one scalar unit the CU has: 80 us for 131072 x 256 against 4 tokens' 2 compares per score in vector ones.)
 #include <algorithm>
 
 #include "pg_rows.h"
@@ -23,8 +25,9 @@ struct BArgs {
   const uint8_t* mask;
   const void* chosen;
   int* counts;
-  unsigned* state;  // [0] which of the two accumulators this evaluation uses; from [4]: 2 x [groups][experts + 2]
+  unsigned* state;  // [0] which of the two accumulators this evaluation uses; from [4]: 2 x [groups][copies][experts + 2]
   int64_t groups, ntiles;
+  unsigned copies;  // of a group's accumulator, taken in turn by its tiles: atomics to one line wait for each other
   int E, k, cbits;
   double lam_e_k;  // lam * experts / k
   double *partials, *out;
@@ -65,109 +68,173 @@ struct Key<double> {
   }
 };
 
-template <typename T, int PL>
-struct __attribute__((packed, aligned(sizeof(T)))) LooseN {
-  T v[PL];
+constexpr int BT = 1024, WAVES = BT / 64;
+
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) LooseV {
+  T v[Elem<T>::N];
 };
-// a lane's experts; those behind the last one are -inf
-template <typename T, int PL>
-__device__ __forceinline__ void load_lane(const T* row, int lane, int E, T (&x)[PL]) {
-  const int e0 = lane * PL;
-  if (e0 + PL <= E) {
-    const LooseN<T, PL> l = *reinterpret_cast<const LooseN<T, PL>*>(row + e0);
+
+// the tokens of a wave's step: L lanes each, NI chunks of V experts
+template <typename T, int L, int NI>
+struct Geom {
+  static constexpr int V = Elem<T>::N, PL = NI * V, TW = 64 / L, STEP = WAVES * TW;  // STEP: tokens between a wave's steps
+  static __device__ __forceinline__ int expert(int i, int j) { return (i * L + (int)(threadIdx.x % L)) * V + j; }
+};
+// scores of token `tk` (of the last one, t1 - 1, if it lies behind it); -inf behind the last expert
+template <typename T, int L, int NI>
+struct Scores {
+  using G = Geom<T, L, NI>;
+  T x[G::PL];
+  uint8_t on;
+  __device__ __forceinline__ void load(const BArgs& a, int64_t tk, int64_t t1) {
+    tk = min(tk, t1 - 1);
+    on = a.mask != nullptr ? a.mask[tk] : (uint8_t)1;
+    const T* row = (const T*)a.x + tk * a.ldx;
 #pragma unroll
-    for (int i = 0; i < PL; ++i) x[i] = l.v[i];
-  } else {
+    for (int i = 0; i < NI; ++i) {
+      const int e = G::expert(i, 0);
+      if (e + G::V <= a.E) {
+        const LooseV<T> l = *reinterpret_cast<const LooseV<T>*>(row + e);
 #pragma unroll
-    for (int i = 0; i < PL; ++i) x[i] = e0 + i < E ? row[e0 + i] : (T)-INFINITY;
+        for (int j = 0; j < G::V; ++j) x[i * G::V + j] = l.v[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < G::V; ++j) x[i * G::V + j] = e + j < a.E ? row[e + j] : (T)-INFINITY;
+      }
+    }
   }
-}
-template <typename T, int PL>
-__device__ __forceinline__ void store_lane(T* row, int lane, int E, const T (&x)[PL]) {
-  const int e0 = lane * PL;
-  if (e0 + PL <= E) {
-    LooseN<T, PL> l;
+};
+template <typename T, int L, int NI>
+__device__ __forceinline__ void store_scores(T* row, int E, const T (&x)[Geom<T, L, NI>::PL]) {
+  using G = Geom<T, L, NI>;
 #pragma unroll
-    for (int i = 0; i < PL; ++i) l.v[i] = x[i];
-    *reinterpret_cast<LooseN<T, PL>*>(row + e0) = l;
-  } else {
+  for (int i = 0; i < NI; ++i) {
+    const int e = G::expert(i, 0);
+    if (e + G::V <= E) {
+      LooseV<T> l;
 #pragma unroll
-    for (int i = 0; i < PL; ++i)
-      if (e0 + i < E) row[e0 + i] = x[i];
+      for (int j = 0; j < G::V; ++j) l.v[j] = x[i * G::V + j];
+      *reinterpret_cast<LooseV<T>*>(row + e) = l;
+    } else {
+#pragma unroll
+      for (int j = 0; j < G::V; ++j)
+        if (e + j < E) row[e + j] = x[i * G::V + j];
+    }
   }
 }
 
-// cnt[i] += the token chooses this lane's expert i.  guess: in, a threshold to start from; out, this token's
-template <typename T, int PL>
-__device__ __forceinline__ void choose(const T (&x)[PL], int k, typename Key<T>::U& guess, int (&cnt)[PL]) {
+// sums and maxima over the L lanes of a token
+template <int CTRL>
+__device__ __forceinline__ int dpp_int(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true);
+}
+template <int L>
+__device__ __forceinline__ int token_sum(int v) {
+  v += dpp_int<0xB1>(v);
+  v += dpp_int<0x4E>(v);
+  v += dpp_int<0x141>(v);
+  if constexpr (L >= 16) v += dpp_int<0x140>(v);
+  if constexpr (L >= 32) v += __shfl_xor(v, 16, 64);
+  if constexpr (L >= 64) v += __shfl_xor(v, 32, 64);
+  return v;
+}
+template <int L, typename C>
+__device__ __forceinline__ C token_sum(C v) {
+  if constexpr (L == 64) return wave_sum(v);
+  v += pg_dpp_mov<0xB1>(v);
+  v += pg_dpp_mov<0x4E>(v);
+  v += pg_dpp_mov<0x141>(v);
+  if constexpr (L >= 16) v += pg_dpp_mov<0x140>(v);
+  if constexpr (L == 32) v += pg_shfl_xor(v, 16);
+  return v;
+}
+template <int L, typename C>
+__device__ __forceinline__ C token_max(C v) {
+  if constexpr (L == 64) return wave_max(v);
+  v = fmx(v, pg_dpp_mov<0xB1>(v));
+  v = fmx(v, pg_dpp_mov<0x4E>(v));
+  v = fmx(v, pg_dpp_mov<0x141>(v));
+  if constexpr (L >= 16) v = fmx(v, pg_dpp_mov<0x140>(v));
+  if constexpr (L == 32) v = fmx(v, pg_shfl_xor(v, 16));
+  return v;
+}
+
+// cnt[i] += the token chooses this lane's i-th expert.  guess: in, a threshold to start from (above 1); out, this token's
+template <typename T, int L, int NI>
+__device__ __forceinline__ void choose(const T (&x)[Geom<T, L, NI>::PL], bool live, int k, typename Key<T>::U& guess, int (&cnt)[Geom<T, L, NI>::PL]) {
   using U = typename Key<T>::U;
+  using G = Geom<T, L, NI>;
+  constexpr int PL = G::PL;
   U key[PL];
 #pragma unroll
-  for (int i = 0; i < PL; ++i) key[i] = Key<T>::of(x[i]);
+  for (int i = 0; i < PL; ++i) key[i] = live ? Key<T>::of(x[i]) : U(0);
   auto count = [&](U t) {
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < PL; ++i) n += __builtin_popcountll(__ballot(key[i] >= t));
-    return n;
+    for (int i = 0; i < PL; ++i) n += key[i] >= t;
+    return token_sum<L>(n);
   };
+  U at = 1;                    // chosen: keys from `at` on
   U lo = 1, hi = Key<T>::top;  // count(lo) >= k > count(hi)
-  int n_hi = 0;
-  if (count(1) <= k) {
-#pragma unroll
-    for (int i = 0; i < PL; ++i) cnt[i] += key[i] != 0;
-    return;
-  }
   U t = guess, step = Key<T>::stride;
+  int n_hi = 0, ties = 0;
   bool below = false, above = false;  // a bound found on that side of the guess
-  while (true) {
+  bool open = count(1) > k;           // (the same in a token's lanes, like everything here but the keys)
+  const bool search = open;
+  while (__any(open)) {
     const int n = count(t);
-    if (n == k) {
-#pragma unroll
-      for (int i = 0; i < PL; ++i) cnt[i] += key[i] >= t;
-      guess = t;
-      return;
-    }
-    if (n > k) {
-      lo = t;
-      below = true;
-    } else {
-      hi = t;
-      n_hi = n;
-      above = true;
-    }
-    if (hi - lo <= 1) break;
-    if (below && above) {
-      t = lo + (hi - lo) / 2;
-    } else if (below) {  // widening upwards
-      t = hi - lo > step ? lo + step : lo + (hi - lo) / 2;
-      step = step > Key<T>::top / 8 ? step : step * 4;
-    } else {
-      t = hi - lo > step ? hi - step : lo + (hi - lo) / 2;
-      step = step > Key<T>::top / 8 ? step : step * 4;
+    if (open) {
+      if (n == k) {
+        at = t;
+        open = false;
+      } else {
+        if (n > k) lo = t, below = true;
+        else hi = t, n_hi = n, above = true;
+        const U gap = hi - lo;
+        if (gap <= 1) {  // scores equal to lo, not all of them chosen
+          at = hi;
+          ties = k - n_hi;
+          open = false;
+        }
+        t = lo + gap / 2;
+        if (!(below && above) && gap > step) t = below ? lo + step : hi - step;  // widening
+        step = step > Key<T>::top / 8 ? step : step * 4;
+      }
     }
   }
-  // several scores equal to lo, not all of them chosen: the lowest indices
-  const int lane = threadIdx.x & 63;
-  int left = k - n_hi;
-  int before = 0;  // equal scores in the lanes in front of this one
+  if (search) guess = at;
 #pragma unroll
-  for (int i = 0; i < PL; ++i) before += __builtin_popcountll(__ballot(key[i] == lo) & ((1ull << lane) - 1));
+  for (int i = 0; i < PL; ++i) cnt[i] += key[i] >= at;
+  if (__any(ties > 0)) {  // the lowest indices among the equal ones
+    const int lane = threadIdx.x & 63;
+    const unsigned long long seg = L == 64 ? ~0ull : ((1ull << (L & 63)) - 1) << (lane & ~(L - 1));
+    int before = 0;  // equal scores of the token in front of this lane's chunk
 #pragma unroll
-  for (int i = 0; i < PL; ++i) {
-    if (key[i] >= hi) ++cnt[i];
-    else if (key[i] == lo) cnt[i] += before++ < left;
+    for (int i = 0; i < NI; ++i) {
+      int lower = 0, all = 0;
+#pragma unroll
+      for (int j = 0; j < G::V; ++j) {
+        const unsigned long long eq = __builtin_amdgcn_ballot_w64(ties > 0 && key[i * G::V + j] == lo) & seg;
+        lower += __builtin_popcountll(eq & ((1ull << lane) - 1));
+        all += __builtin_popcountll(eq);
+      }
+      int mine = before + lower;
+#pragma unroll
+      for (int j = 0; j < G::V; ++j)
+        if (ties > 0 && key[i * G::V + j] == lo) cnt[i * G::V + j] += mine++ < ties;
+      before += all;
+    }
   }
-  guess = lo;
 }
 
-constexpr int BT = 256;
-
 // choices of the tokens [t0, t1) into sc[experts] (LDS), sc[E] unmasked tokens, sc[E + 1] choices out of range
-template <typename T, int PL>
+template <typename T, int L, int NI>
 __device__ __forceinline__ void count_tile(const BArgs& a, int64_t t0, int64_t t1, unsigned* sc) {
+  using G = Geom<T, L, NI>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  unsigned live = 0;
   if (a.chosen != nullptr) {
-    unsigned live = 0;
     for (int64_t t = t0 + threadIdx.x; t < t1; t += BT) {
       if (a.mask != nullptr && !a.mask[t]) continue;
       ++live;
@@ -180,85 +247,90 @@ __device__ __forceinline__ void count_tile(const BArgs& a, int64_t t0, int64_t t
     if (live) atomicAdd(&sc[a.E], live);
     return;
   }
-  int cnt[PL] = {};
+  int cnt[G::PL] = {};
   typename Key<T>::U guess = Key<T>::of((T)1.0f);
-  unsigned live = 0;
-  for (int64_t t = t0 + wave; t < t1; t += BT / 64) {
-    if (a.mask != nullptr && !a.mask[t]) continue;
-    ++live;
-    T x[PL];
-    load_lane<T, PL>((const T*)a.x + t * a.ldx, lane, a.E, x);
-    choose<T, PL>(x, a.k, guess, cnt);
+  int64_t t = t0 + wave * G::TW;
+  if (t >= t1) return;
+  Scores<T, L, NI> s, next;
+  s.load(a, t + lane / L, t1);
+#pragma clang loop unroll(disable)
+  for (; t < t1; t += G::STEP, s = next) {
+    next.load(a, t + G::STEP + lane / L, t1);  // on its way while this one is looked through
+    const bool on = s.on && t + lane / L < t1;
+    live += on;
+    choose<T, L, NI>(s.x, on, a.k, guess, cnt);
   }
 #pragma unroll
-  for (int i = 0; i < PL; ++i)
-    if (cnt[i]) atomicAdd(&sc[lane * PL + i], (unsigned)cnt[i]);
-  if (lane == 0 && live) atomicAdd(&sc[a.E], live);
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < G::V; ++j)
+      if (cnt[i * G::V + j]) atomicAdd(&sc[G::expert(i, j)], (unsigned)cnt[i * G::V + j]);
+  if (lane % L == 0 && live) atomicAdd(&sc[a.E], live);
 }
 
 // gradients of the tokens [t0, t1) from the counts in sc; returns this thread's part of the value
-template <typename T, int PL>
+template <typename T, int L, int NI>
 __device__ __forceinline__ double grad_tile(const BArgs& a, int64_t t0, int64_t t1, const unsigned* sc) {
   using C = typename Elem<T>::C;
+  using G = Geom<T, L, NI>;
+  constexpr int PL = G::PL;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  int64_t t = t0 + wave * G::TW;
+  if (t >= t1) return 0.0;
+  Scores<T, L, NI> b, next;
+  b.load(a, t + lane / L, t1);
   const double n = (double)sc[a.E];
   const double ag = sc[a.E + 1] ? (double)NAN : (n > 0 ? a.lam_e_k / (n * n) : 0.0);
   C c[PL];
 #pragma unroll
-  for (int i = 0; i < PL; ++i) c[i] = lane * PL + i < a.E ? (C)sc[lane * PL + i] : C(0);
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < G::V; ++j) c[i * G::V + j] = G::expert(i, j) < a.E ? (C)sc[G::expert(i, j)] : C(0);
   double sum = 0.0;
-  for (int64_t t = t0 + wave; t < t1; t += BT / 64) {
-    T* gr = (T*)a.g + t * a.ldg;
-    T o[PL];
-    C m = Lim<C>::lowest, x[PL];
-    const bool live = a.mask == nullptr || a.mask[t];
-    if (live) {
-      T xt[PL];
-      load_lane<T, PL>((const T*)a.x + t * a.ldx, lane, a.E, xt);
+#pragma clang loop unroll(disable)
+  for (; t < t1; t += G::STEP, b = next) {
+    next.load(a, t + G::STEP + lane / L, t1);
+    const int64_t tk = t + lane / L;
+    C x[PL], m = Lim<C>::lowest, s = C(0), d = C(0);
 #pragma unroll
-      for (int i = 0; i < PL; ++i) {
-        x[i] = up<T>(xt[i]);
-        m = fmx(m, x[i]);
-      }
-      m = wave_max(m);
-      C s = C(0), d = C(0);
-#pragma unroll
-      for (int i = 0; i < PL; ++i) {
-        x[i] = ex2((x[i] - m) * (C)1.4426950408889634);
-        s += x[i];
-        d += x[i] * c[i];
-      }
-      s = wave_sum(s);
-      d = wave_sum(d);
-      if (s != C(0)) {
-        d /= s;
-        const C f = (C)ag / s;
-#pragma unroll
-        for (int i = 0; i < PL; ++i) o[i] = (T)(f * x[i] * (c[i] - d));
-        sum += ag * (double)d;
-        store_lane<T, PL>(gr, lane, a.E, o);
-        continue;
-      }
+    for (int i = 0; i < PL; ++i) {
+      x[i] = up<T>(b.x[i]);
+      m = fmx(m, x[i]);
     }
+    m = token_max<L>(m);
 #pragma unroll
-    for (int i = 0; i < PL; ++i) o[i] = (T)0.f;
-    store_lane<T, PL>(gr, lane, a.E, o);
+    for (int i = 0; i < PL; ++i) {
+      x[i] = ex2((x[i] - m) * (C)1.4426950408889634);
+      s += x[i];
+      d += x[i] * c[i];
+    }
+    s = token_sum<L>(s);
+    d = token_sum<L>(d);
+    if (tk < t1) {
+      const bool on = b.on != 0 && s != C(0);  // (s = 0: every score -inf)
+      const C dd = d / s, f = (C)ag / s;
+      T o[PL];
+#pragma unroll
+      for (int i = 0; i < PL; ++i) o[i] = on ? (T)(f * x[i] * (c[i] - dd)) : (T)0.f;
+      if (on) sum += ag * (double)dd;
+      store_scores<T, L, NI>((T*)a.g + tk * a.ldg, a.E, o);
+    }
   }
-  return lane == 0 ? sum : 0.0;
+  return lane % L == 0 ? sum : 0.0;
 }
 
-template <typename T, int PL>
+template <typename T, int L, int NI>
 __device__ __forceinline__ void zero_tile(const BArgs& a, int64_t t0, int64_t t1) {
-  T o[PL];
+  T o[Geom<T, L, NI>::PL];
 #pragma unroll
-  for (int i = 0; i < PL; ++i) o[i] = (T)0.f;
-  for (int64_t t = t0 + threadIdx.x / 64; t < t1; t += BT / 64) store_lane<T, PL>((T*)a.g + t * a.ldg, threadIdx.x & 63, a.E, o);
+  for (int i = 0; i < Geom<T, L, NI>::PL; ++i) o[i] = (T)0.f;
+  for (int64_t t = t0 + threadIdx.x / L; t < t1; t += BT / L) store_scores<T, L, NI>((T*)a.g + t * a.ldg, a.E, o);
 }
 
 template <typename C>
 __device__ __forceinline__ bool finish(const BArgs& a, double v) {
   double total;
-  const bool last = sum_workgroups<BT / 64>(v, gridDim.x, blockIdx.x, a.partials, a.counter, total);
+  const bool last = sum_workgroups<WAVES>(v, gridDim.x, blockIdx.x, a.partials, a.counter, total);
   if (last) {
     store_value<C>(total, a.out, a.value);
   }
@@ -266,57 +338,58 @@ __device__ __forceinline__ bool finish(const BArgs& a, double v) {
 }
 
 // first pass: counts into this evaluation's accumulator
-template <typename T, int PL>
+template <typename T, int L, int NI>
 __global__ __launch_bounds__(BT) void balance_count(BArgs a) {
   extern __shared__ unsigned sc[];
   const int W = a.E + 2;
-  unsigned* acc = a.state + 4 + (size_t)(a.state[0] & 1u) * a.groups * W;
+  unsigned* acc = a.state + 4 + (size_t)(a.state[0] & 1u) * a.groups * a.copies * W;
   for (int64_t q = blockIdx.x; q < a.ntiles; q += gridDim.x) {
     const pg_balance_tile tl = a.tiles[q];
     if (tl.group < 0) continue;  // tokens of no group
     for (int i = threadIdx.x; i < W; i += BT) sc[i] = 0;
     __syncthreads();
-    count_tile<T, PL>(a, tl.begin, tl.end, sc);
+    count_tile<T, L, NI>(a, tl.begin, tl.end, sc);
     __syncthreads();
     for (int i = threadIdx.x; i < W; i += BT)
-      if (sc[i]) atomicAdd(&acc[(size_t)tl.group * W + i], sc[i]);
+      if (sc[i]) atomicAdd(&acc[((size_t)tl.group * a.copies + (unsigned)max(tl.part, 0) % a.copies) * W + i], sc[i]);
     __syncthreads();
   }
 }
 
 // second pass: gradients and value; the group's first tile hands the counts out and clears the other accumulator for the
 // next evaluation, the last workgroup to finish turns the two over
-template <typename T, int PL>
+template <typename T, int L, int NI>
 __global__ __launch_bounds__(BT) void balance_grad(BArgs a) {
   extern __shared__ unsigned sc[];
   const int W = a.E + 2;
   const unsigned turn = a.state[0] & 1u;
-  const unsigned* acc = a.state + 4 + (size_t)turn * a.groups * W;
-  unsigned* other = a.state + 4 + (size_t)(turn ^ 1u) * a.groups * W;
+  const unsigned* acc = a.state + 4 + (size_t)turn * a.groups * a.copies * W;
+  unsigned* other = a.state + 4 + (size_t)(turn ^ 1u) * a.groups * a.copies * W;
   double v = 0.0;
   for (int64_t q = blockIdx.x; q < a.ntiles; q += gridDim.x) {
     const pg_balance_tile tl = a.tiles[q];
     if (tl.group < 0) {
-      zero_tile<T, PL>(a, tl.begin, tl.end);
+      zero_tile<T, L, NI>(a, tl.begin, tl.end);
       continue;
     }
     for (int i = threadIdx.x; i < W; i += BT) {
-      const unsigned n = acc[(size_t)tl.group * W + i];
+      unsigned n = 0;
+      for (unsigned p = 0; p < a.copies; ++p) n += acc[((size_t)tl.group * a.copies + p) * W + i];
       sc[i] = n;
       if (tl.part <= 0) {
         if (i < a.E) a.counts[(size_t)tl.group * a.E + i] = (int)n;
-        other[(size_t)tl.group * W + i] = 0;
+        for (unsigned p = 0; p < a.copies; ++p) other[((size_t)tl.group * a.copies + p) * W + i] = 0;
       }
     }
     __syncthreads();
-    v += grad_tile<T, PL>(a, tl.begin, tl.end, sc);
+    v += grad_tile<T, L, NI>(a, tl.begin, tl.end, sc);
     __syncthreads();
   }
   if (finish<typename Elem<T>::C>(a, v)) a.state[0] = turn ^ 1u;
 }
 
 // both passes, a workgroup per group
-template <typename T, int PL>
+template <typename T, int L, int NI>
 __global__ __launch_bounds__(BT) void balance_whole(BArgs a) {
   extern __shared__ unsigned sc[];
   const int W = a.E + 2;
@@ -324,42 +397,48 @@ __global__ __launch_bounds__(BT) void balance_whole(BArgs a) {
   for (int64_t q = blockIdx.x; q < a.ntiles; q += gridDim.x) {
     const pg_balance_tile tl = a.tiles[q];
     if (tl.group < 0) {
-      zero_tile<T, PL>(a, tl.begin, tl.end);
+      zero_tile<T, L, NI>(a, tl.begin, tl.end);
       continue;
     }
     for (int i = threadIdx.x; i < W; i += BT) sc[i] = 0;
     __syncthreads();
-    count_tile<T, PL>(a, tl.begin, tl.end, sc);
+    count_tile<T, L, NI>(a, tl.begin, tl.end, sc);
     __syncthreads();
     for (int i = threadIdx.x; i < a.E; i += BT) a.counts[(size_t)tl.group * a.E + i] = (int)sc[i];
-    v += grad_tile<T, PL>(a, tl.begin, tl.end, sc);
+    v += grad_tile<T, L, NI>(a, tl.begin, tl.end, sc);
     __syncthreads();
   }
   finish<typename Elem<T>::C>(a, v);
 }
 
-template <typename T, int PL>
+template <typename T, int L, int NI>
 pg_status launch(pg_ctx* c, const BArgs& a, bool whole) {
   const size_t lds = (size_t)(a.E + 2) * 4;
-  const unsigned grid = (unsigned)std::min<int64_t>(a.ntiles, std::min(8 * c->num_cu, PG_RED_MAX_BLOCKS));
+  const unsigned grid = (unsigned)std::min<int64_t>(a.ntiles, std::min(2 * c->num_cu, PG_RED_MAX_BLOCKS));
   if (whole) {
-    balance_whole<T, PL><<<grid, BT, lds, c->stream>>>(a);
+    balance_whole<T, L, NI><<<grid, BT, lds, c->stream>>>(a);
     PG_LAUNCH_CHECK();
     return PG_OK;
   }
-  balance_count<T, PL><<<grid, BT, lds, c->stream>>>(a);
+  balance_count<T, L, NI><<<grid, BT, lds, c->stream>>>(a);
   PG_LAUNCH_CHECK();
-  balance_grad<T, PL><<<grid, BT, lds, c->stream>>>(a);
+  balance_grad<T, L, NI><<<grid, BT, lds, c->stream>>>(a);
   PG_LAUNCH_CHECK();
   return PG_OK;
 }
 template <typename T>
 pg_status run(pg_ctx* c, const BArgs& a, bool whole) {
-  if (a.E <= 64) return launch<T, 1>(c, a, whole);
-  if (a.E <= 128) return launch<T, 2>(c, a, whole);
-  if (a.E <= 256) return launch<T, 4>(c, a, whole);
-  if (a.E <= 512) return launch<T, 8>(c, a, whole);
-  return launch<T, 16>(c, a, whole);
+  // a token's lanes: as few as hold it in four registers (bf16, Float16: eight scores a register pair), up to 256 experts in 16 lanes
+  constexpr int V = Elem<T>::N;
+  if (a.E <= 8 * V) return launch<T, 8, 1>(c, a, whole);
+  if (a.E <= 16 * V) return launch<T, 16, 1>(c, a, whole);
+  if (a.E <= 32 * V) return launch<T, 16, 2>(c, a, whole);
+  constexpr int M = 16 / V;  // chunks of 16 scores a lane
+  if constexpr (M >= 4) {
+    if (a.E <= 64 * V) return launch<T, 16, 4>(c, a, whole);
+  }
+  if (a.E <= 32 * M * V) return launch<T, 32, M>(c, a, whole);
+  return launch<T, 64, M>(c, a, whole);
 }
 
 __global__ void balance_zero(double* out, void* value, int f64) {
@@ -401,6 +480,7 @@ extern "C" pg_status pg_balance_value_and_gradient(pg_ctx* c, const pg_balance* 
     a.x = scores, a.g = grad, a.ldx = ld, a.ldg = grad_ld, a.ldc = b->chosen_ld;
     a.tiles = b->tiles, a.mask = (const uint8_t*)b->mask, a.chosen = b->chosen, a.counts = b->counts, a.state = b->state;
     a.groups = b->groups, a.ntiles = b->ntiles, a.E = b->experts, a.k = b->k, a.cbits = b->chosen_bits;
+    a.copies = (unsigned)std::max(b->copies, 1);
     a.lam_e_k = b->lam * b->experts / b->k;
     a.partials = c->red_partials, a.out = out, a.counter = c->red_counter, a.value = value;
     const bool whole = b->whole != 0;

@@ -268,8 +268,8 @@ class DistillationLoss(_RowLoss):
 def _balance_tiles(tokens, offsets, num_cu):
     """([(begin, end, group, part)], whether each group is one tile): the work of one evaluation in pieces of one group each"""
     lengths = [b - a for a, b in zip(offsets, offsets[1:])]
-    whole = max(lengths, default=0) <= 256
-    size = max(1, max(lengths, default=0)) if whole else max(32, -(-tokens // (4 * num_cu)))
+    whole = max(lengths, default=0) <= 128
+    size = max(1, max(lengths, default=0)) if whole else max(128, -(-tokens // (2 * num_cu)))
     tiles = []
     for g, (a, n) in enumerate(zip(offsets, lengths)):
         parts = -(-n // size)
@@ -290,7 +290,7 @@ class BalanceLoss(_RowLoss):
         f(u) = lam sum_g n_experts / (k n_g^2) sum_e c_ge sum_t p_te
 
     lam per group at perfect balance.  The gradient holds the counts fixed, so f is smooth between changes of the choices only,
-    and not convex.  ``mask``: False = the token is not looked at, its gradient is zero, as behind the last group.  After an
+    and not convex.  ``mask``: False = the token counts for nothing and its gradient is zero, as behind the last group.  After an
     evaluation ``counts`` (groups x n_experts, int32, on the device) holds the c of that evaluation: one tensor, overwritten by the next."""
 
     is_convex = False
@@ -337,13 +337,14 @@ class BalanceLoss(_RowLoss):
             tiles_d = torch.from_numpy(packed).to(dev)
             mask, chosen = (None if v is None else v.to(dev) for v in (mask, chosen))
             self._counts = torch.zeros(groups, self.classes, dtype=torch.int32, device=dev)
-            state = torch.zeros(4 + (0 if whole else 2 * groups * (self.classes + 2)), dtype=torch.int32, device=dev)
+            copies = min(32, 1 + max((part for *_, part in tiles), default=0) // 8)  # eight tiles to an accumulator
+            state = torch.zeros(4 + (0 if whole else 2 * groups * copies * (self.classes + 2)), dtype=torch.int32, device=dev)
         self._keep = tiles_d, mask, chosen, state
         ptr = lambda v: None if v is None else v.data_ptr()  # noqa: E731
         self._b = _lib.pg_balance(tokens=self.rows, groups=groups, ntiles=len(tiles), tiles=ptr(tiles_d), mask=ptr(mask), chosen=ptr(chosen),
                                   chosen_ld=0 if chosen is None else (chosen.stride(0) if self.rows > 1 else self.k), counts=ptr(self._counts),
                                   state=ptr(state), experts=self.classes, k=self.k,
-                                  chosen_bits=64 if chosen is not None and chosen.dtype == torch.int64 else 32, whole=whole, lam=self.lam)
+                                  chosen_bits=64 if chosen is not None and chosen.dtype == torch.int64 else 32, whole=whole, copies=copies, lam=self.lam)
         self._bref = C.byref(self._b)
         self._entry = _lib.load().pg_balance_value_and_gradient
 
