@@ -52,6 +52,7 @@ pg_status pg_ctx_create(int32_t device, void* stream, pg_ctx** out) {
   }
   if (hipMalloc(&c->red_partials, sizeof(double) * PG_RED_MAX_BLOCKS * PG_RED_MAX_NS) != hipSuccess ||
       hipMalloc(&c->red_counter, sizeof(unsigned) * 8) != hipSuccess ||
+      hipMalloc(&c->row_tickets, sizeof(unsigned) * 33 * 32) != hipSuccess ||
       hipHostMalloc(&c->hscal, sizeof(double) * PG_S_COUNT, hipHostMallocMapped) != hipSuccess ||
       hipHostGetDevicePointer((void**)&c->dscal, c->hscal, 0) != hipSuccess) {
     pg_set_error("context workspace allocation failed");
@@ -59,6 +60,7 @@ pg_status pg_ctx_create(int32_t device, void* stream, pg_ctx** out) {
     return PG_ERR_ALLOC;
   }
   PG_HIP(hipMemset(c->red_counter, 0, sizeof(unsigned) * 8));
+  PG_HIP(hipMemset(c->row_tickets, 0, sizeof(unsigned) * 33 * 32));
   memset(c->hscal, 0, sizeof(double) * PG_S_COUNT);
   if (const char* v = getenv("PG_TN_TEAM_PLAIN")) c->team_plain_launch = atoi(v) != 0;
   PG_HIP(hipDeviceSynchronize());
@@ -77,6 +79,7 @@ pg_status pg_ctx_destroy(pg_ctx* c) {
   if (c->rteam.wait_stats) (void)hipFree(c->rteam.wait_stats);
   if (c->red_partials) (void)hipFree(c->red_partials);
   if (c->red_counter) (void)hipFree(c->red_counter);
+  if (c->row_tickets) (void)hipFree(c->row_tickets);
   if (c->hscal) (void)hipHostFree(c->hscal);
   if (c->dr_ws) (void)hipFree(c->dr_ws);
   for (hipEvent_t e : c->dr_ev)

@@ -131,6 +131,7 @@ struct pg_ctx {
   // reduction workspace
   double* red_partials = nullptr;  // [PG_RED_MAX_BLOCKS * PG_RED_MAX_NS]
   unsigned* red_counter = nullptr; // [8]
+  unsigned* row_tickets = nullptr; // row losses (pg_rows.h): 1 + 32 tickets, a 128-byte line each
   double* hscal = nullptr;         // [PG_S_COUNT]  scalar block: mapped pinned host memory
   double* dscal = nullptr;         //               ... and its device-side address (kernels store here)
   // collective

@@ -257,9 +257,11 @@ __device__ __forceinline__ C row16_sum(C v) {
 
 // The sum of one Float64 per thread over `n` workgroups of NW waves, of which this is number `me`; every thread of each calls it.
 // Each publishes its own sum with a write-through store and takes a ticket; the last one adds them in their order (the same
-// result whoever is last) and puts the ticket back.  True, with the total, for thread 0 of the last one.
+// result whoever is last) and puts the tickets back.  True, with the total, for thread 0 of the last one.  Tickets of one line
+// are handed out one after the other, some 12 ns each, so the workgroups draw from 32 lines and the last of each line from one more.
+constexpr int TICKET_LINES = 32, TICKET_PITCH = 32;
 template <int NW>
-__device__ __forceinline__ bool sum_workgroups(double v, unsigned n, unsigned me, double* partials, unsigned* ticket, double& total) {
+__device__ __forceinline__ bool sum_workgroups(double v, unsigned n, unsigned me, double* partials, unsigned* tickets, double& total) {
   __shared__ double sw[NW];
   __shared__ int is_last;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -280,14 +282,22 @@ __device__ __forceinline__ bool sum_workgroups(double v, unsigned n, unsigned me
   if (threadIdx.x == 0) {
     __hip_atomic_store(&partials[me], mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    is_last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+    const unsigned line = me % TICKET_LINES, members = (n - line + TICKET_LINES - 1) / TICKET_LINES;
+    unsigned* t = tickets + (1 + line) * TICKET_PITCH;
+    bool last = __hip_atomic_fetch_add(t, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == members - 1;
+    if (last) {
+      __hip_atomic_store(t, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const unsigned lines = n < TICKET_LINES ? n : TICKET_LINES;
+      last = __hip_atomic_fetch_add(tickets, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == lines - 1;
+      if (last) __hip_atomic_store(tickets, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    is_last = last;
   }
   __syncthreads();
   if (!is_last) return false;
   double acc = 0.0;
   for (unsigned i = threadIdx.x; i < n; i += NW * 64) acc += __hip_atomic_load(&partials[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   total = join(acc);
-  if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   return threadIdx.x == 0;
 }
 

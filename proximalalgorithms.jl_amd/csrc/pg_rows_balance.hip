@@ -160,7 +160,11 @@ __device__ __forceinline__ C token_max(C v) {
   return v;
 }
 
-// cnt[i] += the token chooses this lane's i-th expert.  guess: in, a threshold to start from (above 1); out, this token's
+// cnt[i] += the token chooses this lane's i-th expert.  guess: in, a threshold to start from (above 1); out, this token's.
+// A threshold t with more than k keys from it on becomes lo, any other hi; the search ends for a token when exactly k keys lie
+// from hi on, or nothing lies between lo and hi.  A step leads away from the guess, four times as far each time, until there is
+// a bound on both sides, and then to the middle.  Tokens that have ended go through the others' steps unharmed: their bounds
+// only come closer, or, with nothing between, t stays.
 template <typename T, int L, int NI>
 __device__ __forceinline__ void choose(const T (&x)[Geom<T, L, NI>::PL], bool live, int k, typename Key<T>::U& guess, int (&cnt)[Geom<T, L, NI>::PL]) {
   using U = typename Key<T>::U;
@@ -168,44 +172,32 @@ __device__ __forceinline__ void choose(const T (&x)[Geom<T, L, NI>::PL], bool li
   constexpr int PL = G::PL;
   U key[PL];
 #pragma unroll
-  for (int i = 0; i < PL; ++i) key[i] = live ? Key<T>::of(x[i]) : U(0);
-  auto count = [&](U t) {
+  for (int i = 0; i < PL; ++i) key[i] = Key<T>::of(x[i]);
+  U lo = 1, hi = Key<T>::top;  // (no key is 1, none is the top)
+  U t = guess, step = Key<T>::stride;
+  int n_hi = 0;
+  bool up_first = false, first = true;
+  if (!live) lo = t = hi;  // nothing is chosen
+  do {
     int n = 0;
 #pragma unroll
     for (int i = 0; i < PL; ++i) n += key[i] >= t;
-    return token_sum<L>(n);
-  };
-  U at = 1;                    // chosen: keys from `at` on
-  U lo = 1, hi = Key<T>::top;  // count(lo) >= k > count(hi)
-  U t = guess, step = Key<T>::stride;
-  int n_hi = 0, ties = 0;
-  bool below = false, above = false;  // a bound found on that side of the guess
-  bool open = count(1) > k;           // (the same in a token's lanes, like everything here but the keys)
-  const bool search = open;
-  while (__any(open)) {
-    const int n = count(t);
-    if (open) {
-      if (n == k) {
-        at = t;
-        open = false;
-      } else {
-        if (n > k) lo = t, below = true;
-        else hi = t, n_hi = n, above = true;
-        const U gap = hi - lo;
-        if (gap <= 1) {  // scores equal to lo, not all of them chosen
-          at = hi;
-          ties = k - n_hi;
-          open = false;
-        }
-        t = lo + gap / 2;
-        if (!(below && above) && gap > step) t = below ? lo + step : hi - step;  // widening
-        step = step > Key<T>::top / 8 ? step : step * 4;
-      }
-    }
-  }
-  if (search) guess = at;
+    n = token_sum<L>(n);
+    const bool more = n > k;
+    lo = more ? t : lo;
+    hi = more ? hi : t;
+    n_hi = more ? n_hi : n;
+    if (first) up_first = more, first = false;
+    const U half = (hi - lo) >> 1;
+    step = more == up_first ? step : Key<T>::top;
+    const U by = step < half ? step : half;
+    step = step > Key<T>::top / 8 ? step : step << 2;
+    t = more ? t + by : t - by;
+  } while (__any(n_hi != k && hi - lo > 1));
+  const int ties = live ? k - n_hi : 0;  // scores equal to lo that are chosen, if not all of them
+  if (live) guess = hi;
 #pragma unroll
-  for (int i = 0; i < PL; ++i) cnt[i] += key[i] >= at;
+  for (int i = 0; i < PL; ++i) cnt[i] += key[i] >= hi;
   if (__any(ties > 0)) {  // the lowest indices among the equal ones
     const int lane = threadIdx.x & 63;
     const unsigned long long seg = L == 64 ? ~0ull : ((1ull << (L & 63)) - 1) << (lane & ~(L - 1));
@@ -359,7 +351,7 @@ __global__ __launch_bounds__(BT) void balance_count(BArgs a) {
 // second pass: gradients and value; the group's first tile hands the counts out and clears the other accumulator for the
 // next evaluation, the last workgroup to finish turns the two over
 template <typename T, int L, int NI>
-__global__ __launch_bounds__(BT) void balance_grad(BArgs a) {
+__global__ __launch_bounds__(BT, (sizeof(T) == 4 && NI <= 2 ? 8 : 4)) void balance_grad(BArgs a) {
   extern __shared__ unsigned sc[];
   const int W = a.E + 2;
   const unsigned turn = a.state[0] & 1u;
@@ -411,7 +403,7 @@ __global__ __launch_bounds__(BT) void balance_whole(BArgs a) {
   finish<typename Elem<T>::C>(a, v);
 }
 
-template <typename T, int L, int NI>
+template <typename T, int L, int NI, int LG, int NG>
 pg_status launch(pg_ctx* c, const BArgs& a, bool whole) {
   const size_t lds = (size_t)(a.E + 2) * 4;
   const unsigned grid = (unsigned)std::min<int64_t>(a.ntiles, std::min(2 * c->num_cu, PG_RED_MAX_BLOCKS));
@@ -422,23 +414,23 @@ pg_status launch(pg_ctx* c, const BArgs& a, bool whole) {
   }
   balance_count<T, L, NI><<<grid, BT, lds, c->stream>>>(a);
   PG_LAUNCH_CHECK();
-  balance_grad<T, L, NI><<<grid, BT, lds, c->stream>>>(a);
+  balance_grad<T, LG, NG><<<grid, BT, lds, c->stream>>>(a);
   PG_LAUNCH_CHECK();
   return PG_OK;
 }
+// A token's lanes.  Counting: 16, with up to 16 scores each, so that a wave's step serves four tokens; gradients: as many as hold
+// the token in one chunk each (a lane's registers are the number of waves that wait for memory).
 template <typename T>
 pg_status run(pg_ctx* c, const BArgs& a, bool whole) {
-  // a token's lanes: as few as hold it in four registers (bf16, Float16: eight scores a register pair), up to 256 experts in 16 lanes
-  constexpr int V = Elem<T>::N;
-  if (a.E <= 8 * V) return launch<T, 8, 1>(c, a, whole);
-  if (a.E <= 16 * V) return launch<T, 16, 1>(c, a, whole);
-  if (a.E <= 32 * V) return launch<T, 16, 2>(c, a, whole);
-  constexpr int M = 16 / V;  // chunks of 16 scores a lane
+  constexpr int V = Elem<T>::N, M = 16 / V;
+  if (a.E <= 8 * V) return launch<T, 8, 1, 8, 1>(c, a, whole);
+  if (a.E <= 16 * V) return launch<T, 16, 1, 16, 1>(c, a, whole);
+  if (a.E <= 32 * V) return launch<T, 16, 2, 32, 1>(c, a, whole);
   if constexpr (M >= 4) {
-    if (a.E <= 64 * V) return launch<T, 16, 4>(c, a, whole);
+    if (a.E <= 64 * V) return launch<T, 16, 4, 64, 1>(c, a, whole);
   }
-  if (a.E <= 32 * M * V) return launch<T, 32, M>(c, a, whole);
-  return launch<T, 64, M>(c, a, whole);
+  if (a.E <= 32 * M * V) return launch<T, 32, M, 64, M / 2>(c, a, whole);
+  return launch<T, 64, M, 64, M>(c, a, whole);
 }
 
 __global__ void balance_zero(double* out, void* value, int f64) {
@@ -482,7 +474,7 @@ extern "C" pg_status pg_balance_value_and_gradient(pg_ctx* c, const pg_balance* 
     a.groups = b->groups, a.ntiles = b->ntiles, a.E = b->experts, a.k = b->k, a.cbits = b->chosen_bits;
     a.copies = (unsigned)std::max(b->copies, 1);
     a.lam_e_k = b->lam * b->experts / b->k;
-    a.partials = c->red_partials, a.out = out, a.counter = c->red_counter, a.value = value;
+    a.partials = c->red_partials, a.out = out, a.counter = c->row_tickets, a.value = value;
     const bool whole = b->whole != 0;
     if (dtype == PG_F32) PG_TRY(run<float>(c, a, whole));
     else if (dtype == PG_F64) PG_TRY(run<double>(c, a, whole));
