@@ -68,7 +68,9 @@ struct Key<double> {
   }
 };
 
-constexpr int BT = 1024, WAVES = BT / 64;
+// threads of a workgroup: four waves, so that few tokens are spread over many CUs (the search keeps a CU's issue slots busy: 256
+// tokens of 256 experts took 27 us in two workgroups of 1024 threads each); a group of its own workgroup has sixteen
+constexpr int BT = 256, BT_WHOLE = 1024;
 
 template <typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) LooseV {
@@ -78,7 +80,7 @@ struct __attribute__((packed, aligned(sizeof(T)))) LooseV {
 // the tokens of a wave's step: L lanes each, NI chunks of V experts
 template <typename T, int L, int NI>
 struct Geom {
-  static constexpr int V = Elem<T>::N, PL = NI * V, TW = 64 / L, STEP = WAVES * TW;  // STEP: tokens between a wave's steps
+  static constexpr int V = Elem<T>::N, PL = NI * V, TW = 64 / L;
   static __device__ __forceinline__ int expert(int i, int j) { return (i * L + (int)(threadIdx.x % L)) * V + j; }
 };
 // scores of token `tk` (of the last one, t1 - 1, if it lies behind it); -inf behind the last expert
@@ -131,9 +133,9 @@ __device__ __forceinline__ int dpp_int(int v) {
 }
 template <int L>
 __device__ __forceinline__ int token_sum(int v) {
-  v += dpp_int<0xB1>(v);
-  v += dpp_int<0x4E>(v);
-  v += dpp_int<0x141>(v);
+  if constexpr (L >= 2) v += dpp_int<0xB1>(v);
+  if constexpr (L >= 4) v += dpp_int<0x4E>(v);
+  if constexpr (L >= 8) v += dpp_int<0x141>(v);
   if constexpr (L >= 16) v += dpp_int<0x140>(v);
   if constexpr (L >= 32) v += __shfl_xor(v, 16, 64);
   if constexpr (L >= 64) v += __shfl_xor(v, 32, 64);
@@ -142,9 +144,9 @@ __device__ __forceinline__ int token_sum(int v) {
 template <int L, typename C>
 __device__ __forceinline__ C token_sum(C v) {
   if constexpr (L == 64) return wave_sum(v);
-  v += pg_dpp_mov<0xB1>(v);
-  v += pg_dpp_mov<0x4E>(v);
-  v += pg_dpp_mov<0x141>(v);
+  if constexpr (L >= 2) v += pg_dpp_mov<0xB1>(v);
+  if constexpr (L >= 4) v += pg_dpp_mov<0x4E>(v);
+  if constexpr (L >= 8) v += pg_dpp_mov<0x141>(v);
   if constexpr (L >= 16) v += pg_dpp_mov<0x140>(v);
   if constexpr (L == 32) v += pg_shfl_xor(v, 16);
   return v;
@@ -152,9 +154,9 @@ __device__ __forceinline__ C token_sum(C v) {
 template <int L, typename C>
 __device__ __forceinline__ C token_max(C v) {
   if constexpr (L == 64) return wave_max(v);
-  v = fmx(v, pg_dpp_mov<0xB1>(v));
-  v = fmx(v, pg_dpp_mov<0x4E>(v));
-  v = fmx(v, pg_dpp_mov<0x141>(v));
+  if constexpr (L >= 2) v = fmx(v, pg_dpp_mov<0xB1>(v));
+  if constexpr (L >= 4) v = fmx(v, pg_dpp_mov<0x4E>(v));
+  if constexpr (L >= 8) v = fmx(v, pg_dpp_mov<0x141>(v));
   if constexpr (L >= 16) v = fmx(v, pg_dpp_mov<0x140>(v));
   if constexpr (L == 32) v = fmx(v, pg_shfl_xor(v, 16));
   return v;
@@ -221,13 +223,14 @@ __device__ __forceinline__ void choose(const T (&x)[Geom<T, L, NI>::PL], bool li
 }
 
 // choices of the tokens [t0, t1) into sc[experts] (LDS), sc[E] unmasked tokens, sc[E + 1] choices out of range
-template <typename T, int L, int NI>
+template <typename T, int L, int NI, int NT>
 __device__ __forceinline__ void count_tile(const BArgs& a, int64_t t0, int64_t t1, unsigned* sc) {
   using G = Geom<T, L, NI>;
+  constexpr int STEP = NT / L;  // tokens between a wave's steps
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   unsigned live = 0;
   if (a.chosen != nullptr) {
-    for (int64_t t = t0 + threadIdx.x; t < t1; t += BT) {
+    for (int64_t t = t0 + threadIdx.x; t < t1; t += NT) {
       if (a.mask != nullptr && !a.mask[t]) continue;
       ++live;
       for (int j = 0; j < a.k; ++j) {
@@ -246,8 +249,8 @@ __device__ __forceinline__ void count_tile(const BArgs& a, int64_t t0, int64_t t
   Scores<T, L, NI> s, next;
   s.load(a, t + lane / L, t1);
 #pragma clang loop unroll(disable)
-  for (; t < t1; t += G::STEP, s = next) {
-    next.load(a, t + G::STEP + lane / L, t1);  // on its way while this one is looked through
+  for (; t < t1; t += STEP, s = next) {
+    next.load(a, t + STEP + lane / L, t1);  // on its way while this one is looked through
     const bool on = s.on && t + lane / L < t1;
     live += on;
     choose<T, L, NI>(s.x, on, a.k, guess, cnt);
@@ -261,11 +264,11 @@ __device__ __forceinline__ void count_tile(const BArgs& a, int64_t t0, int64_t t
 }
 
 // gradients of the tokens [t0, t1) from the counts in sc; returns this thread's part of the value
-template <typename T, int L, int NI>
+template <typename T, int L, int NI, int NT>
 __device__ __forceinline__ double grad_tile(const BArgs& a, int64_t t0, int64_t t1, const unsigned* sc) {
   using C = typename Elem<T>::C;
   using G = Geom<T, L, NI>;
-  constexpr int PL = G::PL;
+  constexpr int PL = G::PL, STEP = NT / L;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   int64_t t = t0 + wave * G::TW;
   if (t >= t1) return 0.0;
@@ -280,8 +283,8 @@ __device__ __forceinline__ double grad_tile(const BArgs& a, int64_t t0, int64_t 
     for (int j = 0; j < G::V; ++j) c[i * G::V + j] = G::expert(i, j) < a.E ? (C)sc[G::expert(i, j)] : C(0);
   double sum = 0.0;
 #pragma clang loop unroll(disable)
-  for (; t < t1; t += G::STEP, b = next) {
-    next.load(a, t + G::STEP + lane / L, t1);
+  for (; t < t1; t += STEP, b = next) {
+    next.load(a, t + STEP + lane / L, t1);
     const int64_t tk = t + lane / L;
     C x[PL], m = Lim<C>::lowest, s = C(0), d = C(0);
 #pragma unroll
@@ -311,18 +314,18 @@ __device__ __forceinline__ double grad_tile(const BArgs& a, int64_t t0, int64_t 
   return lane % L == 0 ? sum : 0.0;
 }
 
-template <typename T, int L, int NI>
+template <typename T, int L, int NI, int NT>
 __device__ __forceinline__ void zero_tile(const BArgs& a, int64_t t0, int64_t t1) {
   T o[Geom<T, L, NI>::PL];
 #pragma unroll
   for (int i = 0; i < Geom<T, L, NI>::PL; ++i) o[i] = (T)0.f;
-  for (int64_t t = t0 + threadIdx.x / L; t < t1; t += BT / L) store_scores<T, L, NI>((T*)a.g + t * a.ldg, a.E, o);
+  for (int64_t t = t0 + threadIdx.x / L; t < t1; t += NT / L) store_scores<T, L, NI>((T*)a.g + t * a.ldg, a.E, o);
 }
 
-template <typename C>
+template <typename C, int NT>
 __device__ __forceinline__ bool finish(const BArgs& a, double v) {
   double total;
-  const bool last = sum_workgroups<WAVES>(v, gridDim.x, blockIdx.x, a.partials, a.counter, total);
+  const bool last = sum_workgroups<NT / 64>(v, gridDim.x, blockIdx.x, a.partials, a.counter, total);
   if (last) {
     store_value<C>(total, a.out, a.value);
   }
@@ -340,7 +343,7 @@ __global__ __launch_bounds__(BT) void balance_count(BArgs a) {
     if (tl.group < 0) continue;  // tokens of no group
     for (int i = threadIdx.x; i < W; i += BT) sc[i] = 0;
     __syncthreads();
-    count_tile<T, L, NI>(a, tl.begin, tl.end, sc);
+    count_tile<T, L, NI, BT>(a, tl.begin, tl.end, sc);
     __syncthreads();
     for (int i = threadIdx.x; i < W; i += BT)
       if (sc[i]) atomicAdd(&acc[((size_t)tl.group * a.copies + (unsigned)max(tl.part, 0) % a.copies) * W + i], sc[i]);
@@ -351,7 +354,7 @@ __global__ __launch_bounds__(BT) void balance_count(BArgs a) {
 // second pass: gradients and value; the group's first tile hands the counts out and clears the other accumulator for the
 // next evaluation, the last workgroup to finish turns the two over
 template <typename T, int L, int NI>
-__global__ __launch_bounds__(BT, (sizeof(T) == 4 && NI <= 2 ? 8 : 4)) void balance_grad(BArgs a) {
+__global__ __launch_bounds__(BT) void balance_grad(BArgs a) {
   extern __shared__ unsigned sc[];
   const int W = a.E + 2;
   const unsigned turn = a.state[0] & 1u;
@@ -361,7 +364,7 @@ __global__ __launch_bounds__(BT, (sizeof(T) == 4 && NI <= 2 ? 8 : 4)) void balan
   for (int64_t q = blockIdx.x; q < a.ntiles; q += gridDim.x) {
     const pg_balance_tile tl = a.tiles[q];
     if (tl.group < 0) {
-      zero_tile<T, L, NI>(a, tl.begin, tl.end);
+      zero_tile<T, L, NI, BT>(a, tl.begin, tl.end);
       continue;
     }
     for (int i = threadIdx.x; i < W; i += BT) {
@@ -374,41 +377,41 @@ __global__ __launch_bounds__(BT, (sizeof(T) == 4 && NI <= 2 ? 8 : 4)) void balan
       }
     }
     __syncthreads();
-    v += grad_tile<T, L, NI>(a, tl.begin, tl.end, sc);
+    v += grad_tile<T, L, NI, BT>(a, tl.begin, tl.end, sc);
     __syncthreads();
   }
-  if (finish<typename Elem<T>::C>(a, v)) a.state[0] = turn ^ 1u;
+  if (finish<typename Elem<T>::C, BT>(a, v)) a.state[0] = turn ^ 1u;
 }
 
 // both passes, a workgroup per group
 template <typename T, int L, int NI>
-__global__ __launch_bounds__(BT) void balance_whole(BArgs a) {
+__global__ __launch_bounds__(BT_WHOLE) void balance_whole(BArgs a) {
   extern __shared__ unsigned sc[];
   const int W = a.E + 2;
   double v = 0.0;
   for (int64_t q = blockIdx.x; q < a.ntiles; q += gridDim.x) {
     const pg_balance_tile tl = a.tiles[q];
     if (tl.group < 0) {
-      zero_tile<T, L, NI>(a, tl.begin, tl.end);
+      zero_tile<T, L, NI, BT_WHOLE>(a, tl.begin, tl.end);
       continue;
     }
-    for (int i = threadIdx.x; i < W; i += BT) sc[i] = 0;
+    for (int i = threadIdx.x; i < W; i += BT_WHOLE) sc[i] = 0;
     __syncthreads();
-    count_tile<T, L, NI>(a, tl.begin, tl.end, sc);
+    count_tile<T, L, NI, BT_WHOLE>(a, tl.begin, tl.end, sc);
     __syncthreads();
-    for (int i = threadIdx.x; i < a.E; i += BT) a.counts[(size_t)tl.group * a.E + i] = (int)sc[i];
-    v += grad_tile<T, L, NI>(a, tl.begin, tl.end, sc);
+    for (int i = threadIdx.x; i < a.E; i += BT_WHOLE) a.counts[(size_t)tl.group * a.E + i] = (int)sc[i];
+    v += grad_tile<T, L, NI, BT_WHOLE>(a, tl.begin, tl.end, sc);
     __syncthreads();
   }
-  finish<typename Elem<T>::C>(a, v);
+  finish<typename Elem<T>::C, BT_WHOLE>(a, v);
 }
 
 template <typename T, int L, int NI, int LG, int NG>
 pg_status launch(pg_ctx* c, const BArgs& a, bool whole) {
   const size_t lds = (size_t)(a.E + 2) * 4;
-  const unsigned grid = (unsigned)std::min<int64_t>(a.ntiles, std::min(2 * c->num_cu, PG_RED_MAX_BLOCKS));
+  const unsigned grid = (unsigned)std::min<int64_t>(a.ntiles, std::min(8 * c->num_cu, PG_RED_MAX_BLOCKS));
   if (whole) {
-    balance_whole<T, L, NI><<<grid, BT, lds, c->stream>>>(a);
+    balance_whole<T, L, NI><<<grid, BT_WHOLE, lds, c->stream>>>(a);
     PG_LAUNCH_CHECK();
     return PG_OK;
   }
@@ -418,11 +421,14 @@ pg_status launch(pg_ctx* c, const BArgs& a, bool whole) {
   PG_LAUNCH_CHECK();
   return PG_OK;
 }
-// A token's lanes.  Counting: 16, with up to 16 scores each, so that a wave's step serves four tokens; gradients: as many as hold
+// A token's lanes.  Counting: at most 16 where that leaves a lane at most 16 scores, so that a wave's step serves four tokens and more; gradients: as many as hold
 // the token in one chunk each (a lane's registers are the number of waves that wait for memory).
 template <typename T>
 pg_status run(pg_ctx* c, const BArgs& a, bool whole) {
   constexpr int V = Elem<T>::N, M = 16 / V;
+  if (a.E <= V) return launch<T, 1, 1, 1, 1>(c, a, whole);
+  if (a.E <= 2 * V) return launch<T, 2, 1, 2, 1>(c, a, whole);
+  if (a.E <= 4 * V) return launch<T, 4, 1, 4, 1>(c, a, whole);
   if (a.E <= 8 * V) return launch<T, 8, 1, 8, 1>(c, a, whole);
   if (a.E <= 16 * V) return launch<T, 16, 1, 16, 1>(c, a, whole);
   if (a.E <= 32 * V) return launch<T, 16, 2, 32, 1>(c, a, whole);
@@ -455,6 +461,7 @@ extern "C" pg_status pg_balance_value_and_gradient(pg_ctx* c, const pg_balance* 
   if (any) {
     PG_REQUIRE(scores != nullptr && grad != nullptr, "null rows");
     PG_REQUIRE(b->tiles != nullptr && (b->counts != nullptr || b->groups == 0) && b->state != nullptr, "null plan");
+    PG_REQUIRE(b->whole || b->copies >= 1, "copies must be at least 1");
     PG_REQUIRE((ld >= b->experts && grad_ld >= b->experts) || b->tokens == 1, "rows overlap: ld below the number of experts");
     PG_REQUIRE(scores != grad || ld == grad_ld || b->tokens == 1, "a gradient in the scores' own buffer needs the scores' ld");
     PG_REQUIRE(((uintptr_t)scores | (uintptr_t)grad) % dtype_size(dtype) == 0, "scores or gradient not aligned to their element");
@@ -472,7 +479,7 @@ extern "C" pg_status pg_balance_value_and_gradient(pg_ctx* c, const pg_balance* 
     a.x = scores, a.g = grad, a.ldx = ld, a.ldg = grad_ld, a.ldc = b->chosen_ld;
     a.tiles = b->tiles, a.mask = (const uint8_t*)b->mask, a.chosen = b->chosen, a.counts = b->counts, a.state = b->state;
     a.groups = b->groups, a.ntiles = b->ntiles, a.E = b->experts, a.k = b->k, a.cbits = b->chosen_bits;
-    a.copies = (unsigned)std::max(b->copies, 1);
+    a.copies = (unsigned)b->copies;
     a.lam_e_k = b->lam * b->experts / b->k;
     a.partials = c->red_partials, a.out = out, a.counter = c->row_tickets, a.value = value;
     const bool whole = b->whole != 0;

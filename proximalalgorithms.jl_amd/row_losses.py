@@ -265,16 +265,22 @@ class DistillationLoss(_RowLoss):
             _lib.check(status)
 
 
-def _balance_tiles(tokens, offsets, num_cu):
-    """([(begin, end, group, part)], whether each group is one tile): the work of one evaluation in pieces of one group each"""
+def _balance_tiles(tokens, experts, offsets, num_cu):
+    """([(begin, end, group, part)], whether each group is one tile): the work of one evaluation in pieces of one group each.
+
+    Small groups take a workgroup each and one launch; 64 tokens of 64 experts take 7 us that way and 9 in tiles, 64 of 256 experts 15
+    and 13.5.  Else a tile is four waves' work, at least a step of theirs: four tiles per compute unit (131072 x 256: 107 us; two 117,
+    eight 110), no fewer than 16 tokens in one (256 x 256: 14 us; 32 tokens 18, 64 tokens 25)."""
     lengths = [b - a for a, b in zip(offsets, offsets[1:])]
-    whole = max(lengths, default=0) <= 128
-    size = max(1, max(lengths, default=0)) if whole else max(128, -(-tokens // (2 * num_cu)))
+    longest = max(lengths, default=0)
+    whole = longest * experts <= 4096
+    size = max(1, longest) if whole else max(16, -(-tokens // (4 * num_cu)))
     tiles = []
     for g, (a, n) in enumerate(zip(offsets, lengths)):
         parts = -(-n // size)
         for q in range(parts):
             tiles.append((a + n * q // parts, a + n * (q + 1) // parts, g, -1 if parts == 1 else q))
+    size = max(size, 16)
     for a in range(offsets[-1], tokens, size):  # behind the last group
         tiles.append((a, min(tokens, a + size), -1, 0))
     return tiles, whole
@@ -331,13 +337,13 @@ class BalanceLoss(_RowLoss):
         self.ctx = _common_device((mask, chosen), ctx)
         dev = self.ctx.torch_device
         groups = len(offsets) - 1
-        tiles, whole = _balance_tiles(self.rows, offsets, self.ctx.device_info()["compute_units"])
+        tiles, whole = _balance_tiles(self.rows, self.classes, offsets, self.ctx.device_info()["compute_units"])
         packed = np.array([(b, e, (g & 0xFFFFFFFF) | ((part & 0xFFFFFFFF) << 32)) for b, e, g, part in tiles], np.uint64).reshape(-1, 3).view(np.int64)
         with _Ordered(self.ctx):
             tiles_d = torch.from_numpy(packed).to(dev)
             mask, chosen = (None if v is None else v.to(dev) for v in (mask, chosen))
             self._counts = torch.zeros(groups, self.classes, dtype=torch.int32, device=dev)
-            copies = min(32, 1 + max((part for *_, part in tiles), default=0) // 8)  # eight tiles to an accumulator
+            copies = min(16, 1 + max((max(part, 0) for *_, part in tiles), default=0) // 16)  # some sixteen tiles to an accumulator
             state = torch.zeros(4 + (0 if whole else 2 * groups * copies * (self.classes + 2)), dtype=torch.int32, device=dev)
         self._keep = tiles_d, mask, chosen, state
         ptr = lambda v: None if v is None else v.data_ptr()  # noqa: E731
