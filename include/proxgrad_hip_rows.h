@@ -80,6 +80,7 @@ typedef struct pg_balance_tile {
 } pg_balance_tile;
 typedef struct pg_balance {
   int64_t tokens, groups, ntiles; /* tokens < 2^31 */
+  int64_t tile_tokens;            /* tiles == NULL: one group of all tokens, in tiles of this many (the last one shorter) */
   const pg_balance_tile* tiles;   /* device; every token in at most one tile, a group's tiles in any order */
   const void* mask;               /* [tokens] bytes, 0 = masked; NULL: none */
   const void* chosen;             /* [tokens x k] int32 or int64; NULL: the k highest */
@@ -88,7 +89,7 @@ typedef struct pg_balance {
   uint32_t* state;  /* device, 4 + 2 * groups * copies * (experts + 2) words, zero before the first evaluation: this loss's own */
   int32_t experts, k, chosen_bits; /* 1 <= k <= experts <= 1024 */
   int32_t whole;                   /* every tile is a whole group: one launch (state: 4 words) */
-  int32_t copies, reserved;        /* accumulators per group that its tiles take in turn, >= 1 */
+  int32_t copies, reserved;        /* accumulators per group that its tiles take in turn, 1 .. 16 */
   double lam;
 } pg_balance;
 

@@ -182,7 +182,7 @@ class pg_balance_tile(C.Structure):
 
 
 class pg_balance(C.Structure):
-    _fields_ = [("tokens", C.c_int64), ("groups", C.c_int64), ("ntiles", C.c_int64), ("tiles", C.c_void_p), ("mask", C.c_void_p),
+    _fields_ = [("tokens", C.c_int64), ("groups", C.c_int64), ("ntiles", C.c_int64), ("tile_tokens", C.c_int64), ("tiles", C.c_void_p), ("mask", C.c_void_p),
                 ("chosen", C.c_void_p), ("chosen_ld", C.c_int64), ("counts", C.c_void_p), ("state", C.c_void_p), ("experts", C.c_int32),
                 ("k", C.c_int32), ("chosen_bits", C.c_int32), ("whole", C.c_int32), ("copies", C.c_int32), ("reserved", C.c_int32), ("lam", C.c_double)]
 

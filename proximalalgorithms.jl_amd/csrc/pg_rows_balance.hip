@@ -26,7 +26,7 @@ struct BArgs {
   const void* chosen;
   int* counts;
   unsigned* state;  // [0] which of the two accumulators this evaluation uses; from [4]: 2 x [groups][copies][experts + 2]
-  int64_t groups, ntiles;
+  int64_t groups, ntiles, tokens, tile_tokens;
   unsigned copies;  // of a group's accumulator, taken in turn by its tiles: atomics to one line wait for each other
   int E, k, cbits;
   double lam_e_k;  // lam * experts / k
@@ -71,6 +71,7 @@ struct Key<double> {
 // threads of a workgroup: four waves, so that few tokens are spread over many CUs (the search keeps a CU's issue slots busy: 256
 // tokens of 256 experts took 27 us in two workgroups of 1024 threads each); a group of its own workgroup has sixteen
 constexpr int BT = 256, BT_WHOLE = 1024;
+constexpr unsigned MAX_COPIES = 16;
 
 template <typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) LooseV {
@@ -117,7 +118,9 @@ __device__ __forceinline__ void store_scores(T* row, int E, const T (&x)[Geom<T,
       LooseV<T> l;
 #pragma unroll
       for (int j = 0; j < G::V; ++j) l.v[j] = x[i * G::V + j];
-      *reinterpret_cast<LooseV<T>*>(row + e) = l;
+      // non-temporal: nobody reads a gradient here, and the scores, read twice, keep their place in the caches (131072 x 256: 99 us, 106 without)
+      typedef u32x4 __attribute__((aligned(2))) Anywhere;
+      __builtin_nontemporal_store(__builtin_bit_cast(u32x4, l), reinterpret_cast<Anywhere*>(row + e));
     } else {
 #pragma unroll
       for (int j = 0; j < G::V; ++j)
@@ -222,6 +225,14 @@ __device__ __forceinline__ void choose(const T (&x)[Geom<T, L, NI>::PL], bool li
   }
 }
 
+__device__ __forceinline__ pg_balance_tile tile_at(const BArgs& a, int64_t q) {
+  if (a.tiles != nullptr) return a.tiles[q];
+  pg_balance_tile t;
+  t.begin = q * a.tile_tokens, t.end = min(t.begin + a.tile_tokens, a.tokens);
+  t.group = 0, t.part = (int)q;
+  return t;
+}
+
 // choices of the tokens [t0, t1) into sc[experts] (LDS), sc[E] unmasked tokens, sc[E + 1] choices out of range
 template <typename T, int L, int NI, int NT>
 __device__ __forceinline__ void count_tile(const BArgs& a, int64_t t0, int64_t t1, unsigned* sc) {
@@ -263,17 +274,22 @@ __device__ __forceinline__ void count_tile(const BArgs& a, int64_t t0, int64_t t
   if (lane % L == 0 && live) atomicAdd(&sc[a.E], live);
 }
 
-// gradients of the tokens [t0, t1) from the counts in sc; returns this thread's part of the value
+// the first tokens of a wave in a tile
+template <typename T, int L, int NI>
+__device__ __forceinline__ void first_scores(const BArgs& a, int64_t t0, int64_t t1, Scores<T, L, NI>& b) {
+  if (t0 + (int64_t)(threadIdx.x / 64) * (64 / L) < t1) b.load(a, t0 + threadIdx.x / L, t1);
+}
+
+// gradients of the tokens [t0, t1) from the counts in sc; b: first_scores; returns this thread's part of the value
 template <typename T, int L, int NI, int NT>
-__device__ __forceinline__ double grad_tile(const BArgs& a, int64_t t0, int64_t t1, const unsigned* sc) {
+__device__ __forceinline__ double grad_tile(const BArgs& a, int64_t t0, int64_t t1, const unsigned* sc, Scores<T, L, NI> b) {
   using C = typename Elem<T>::C;
   using G = Geom<T, L, NI>;
   constexpr int PL = G::PL, STEP = NT / L;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   int64_t t = t0 + wave * G::TW;
   if (t >= t1) return 0.0;
-  Scores<T, L, NI> b, next;
-  b.load(a, t + lane / L, t1);
+  Scores<T, L, NI> next;
   const double n = (double)sc[a.E];
   const double ag = sc[a.E + 1] ? (double)NAN : (n > 0 ? a.lam_e_k / (n * n) : 0.0);
   C c[PL];
@@ -339,7 +355,7 @@ __global__ __launch_bounds__(BT) void balance_count(BArgs a) {
   const int W = a.E + 2;
   unsigned* acc = a.state + 4 + (size_t)(a.state[0] & 1u) * a.groups * a.copies * W;
   for (int64_t q = blockIdx.x; q < a.ntiles; q += gridDim.x) {
-    const pg_balance_tile tl = a.tiles[q];
+    const pg_balance_tile tl = tile_at(a, q);
     if (tl.group < 0) continue;  // tokens of no group
     for (int i = threadIdx.x; i < W; i += BT) sc[i] = 0;
     __syncthreads();
@@ -362,14 +378,23 @@ __global__ __launch_bounds__(BT) void balance_grad(BArgs a) {
   unsigned* other = a.state + 4 + (size_t)(turn ^ 1u) * a.groups * a.copies * W;
   double v = 0.0;
   for (int64_t q = blockIdx.x; q < a.ntiles; q += gridDim.x) {
-    const pg_balance_tile tl = a.tiles[q];
+    const pg_balance_tile tl = tile_at(a, q);
     if (tl.group < 0) {
       zero_tile<T, L, NI, BT>(a, tl.begin, tl.end);
       continue;
     }
+    Scores<T, L, NI> b;
+    first_scores<T, L, NI>(a, tl.begin, tl.end, b);  // on their way while the counts are added up
     for (int i = threadIdx.x; i < W; i += BT) {
-      unsigned n = 0;
-      for (unsigned p = 0; p < a.copies; ++p) n += acc[((size_t)tl.group * a.copies + p) * W + i];
+      const unsigned* mine = acc + (size_t)tl.group * a.copies * W + i;
+      unsigned n = mine[0];
+      if (a.copies > 1) {  // all of them asked for at once
+#pragma unroll
+        for (unsigned p = 1; p < MAX_COPIES; ++p) {
+          const unsigned m = mine[(size_t)min(p, a.copies - 1) * W];
+          n += p < a.copies ? m : 0u;
+        }
+      }
       sc[i] = n;
       if (tl.part <= 0) {
         if (i < a.E) a.counts[(size_t)tl.group * a.E + i] = (int)n;
@@ -377,7 +402,7 @@ __global__ __launch_bounds__(BT) void balance_grad(BArgs a) {
       }
     }
     __syncthreads();
-    v += grad_tile<T, L, NI, BT>(a, tl.begin, tl.end, sc);
+    v += grad_tile<T, L, NI, BT>(a, tl.begin, tl.end, sc, b);
     __syncthreads();
   }
   if (finish<typename Elem<T>::C, BT>(a, v)) a.state[0] = turn ^ 1u;
@@ -390,7 +415,7 @@ __global__ __launch_bounds__(BT_WHOLE) void balance_whole(BArgs a) {
   const int W = a.E + 2;
   double v = 0.0;
   for (int64_t q = blockIdx.x; q < a.ntiles; q += gridDim.x) {
-    const pg_balance_tile tl = a.tiles[q];
+    const pg_balance_tile tl = tile_at(a, q);
     if (tl.group < 0) {
       zero_tile<T, L, NI, BT_WHOLE>(a, tl.begin, tl.end);
       continue;
@@ -400,7 +425,9 @@ __global__ __launch_bounds__(BT_WHOLE) void balance_whole(BArgs a) {
     count_tile<T, L, NI, BT_WHOLE>(a, tl.begin, tl.end, sc);
     __syncthreads();
     for (int i = threadIdx.x; i < a.E; i += BT_WHOLE) a.counts[(size_t)tl.group * a.E + i] = (int)sc[i];
-    v += grad_tile<T, L, NI, BT_WHOLE>(a, tl.begin, tl.end, sc);
+    Scores<T, L, NI> b;
+    first_scores<T, L, NI>(a, tl.begin, tl.end, b);
+    v += grad_tile<T, L, NI, BT_WHOLE>(a, tl.begin, tl.end, sc, b);
     __syncthreads();
   }
   finish<typename Elem<T>::C, BT_WHOLE>(a, v);
@@ -460,8 +487,10 @@ extern "C" pg_status pg_balance_value_and_gradient(pg_ctx* c, const pg_balance* 
   const bool any = b->tokens > 0 && b->ntiles > 0;
   if (any) {
     PG_REQUIRE(scores != nullptr && grad != nullptr, "null rows");
-    PG_REQUIRE(b->tiles != nullptr && (b->counts != nullptr || b->groups == 0) && b->state != nullptr, "null plan");
-    PG_REQUIRE(b->whole || b->copies >= 1, "copies must be at least 1");
+    PG_REQUIRE(b->tiles != nullptr || (b->groups == 1 && b->tile_tokens > 0 && b->ntiles == (b->tokens + b->tile_tokens - 1) / b->tile_tokens),
+               "without tiles: one group, ntiles of tile_tokens tokens");
+    PG_REQUIRE((b->counts != nullptr || b->groups == 0) && b->state != nullptr, "null plan");
+    PG_REQUIRE(b->whole || (b->copies >= 1 && b->copies <= (int)MAX_COPIES), "copies must be between 1 and 16");
     PG_REQUIRE((ld >= b->experts && grad_ld >= b->experts) || b->tokens == 1, "rows overlap: ld below the number of experts");
     PG_REQUIRE(scores != grad || ld == grad_ld || b->tokens == 1, "a gradient in the scores' own buffer needs the scores' ld");
     PG_REQUIRE(((uintptr_t)scores | (uintptr_t)grad) % dtype_size(dtype) == 0, "scores or gradient not aligned to their element");
@@ -478,7 +507,7 @@ extern "C" pg_status pg_balance_value_and_gradient(pg_ctx* c, const pg_balance* 
     BArgs a{};
     a.x = scores, a.g = grad, a.ldx = ld, a.ldg = grad_ld, a.ldc = b->chosen_ld;
     a.tiles = b->tiles, a.mask = (const uint8_t*)b->mask, a.chosen = b->chosen, a.counts = b->counts, a.state = b->state;
-    a.groups = b->groups, a.ntiles = b->ntiles, a.E = b->experts, a.k = b->k, a.cbits = b->chosen_bits;
+    a.groups = b->groups, a.ntiles = b->ntiles, a.tokens = b->tokens, a.tile_tokens = b->tile_tokens, a.E = b->experts, a.k = b->k, a.cbits = b->chosen_bits;
     a.copies = (unsigned)b->copies;
     a.lam_e_k = b->lam * b->experts / b->k;
     a.partials = c->red_partials, a.out = out, a.counter = c->row_tickets, a.value = value;

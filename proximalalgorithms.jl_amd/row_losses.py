@@ -266,24 +266,26 @@ class DistillationLoss(_RowLoss):
 
 
 def _balance_tiles(tokens, experts, offsets, num_cu):
-    """([(begin, end, group, part)], whether each group is one tile): the work of one evaluation in pieces of one group each.
+    """(rows of (begin, end, group, part), tokens of a tile, whether each group is one tile): an evaluation in pieces of one group each.
 
     Small groups take a workgroup each and one launch; 64 tokens of 64 experts take 7 us that way and 9 in tiles, 64 of 256 experts 15
     and 13.5.  Else a tile is four waves' work, at least a step of theirs: four tiles per compute unit (131072 x 256: 107 us; two 117,
     eight 110), no fewer than 16 tokens in one (256 x 256: 14 us; 32 tokens 18, 64 tokens 25)."""
-    lengths = [b - a for a, b in zip(offsets, offsets[1:])]
-    longest = max(lengths, default=0)
+    offsets = np.asarray(offsets, np.int64)
+    lengths = np.diff(offsets)
+    longest = int(lengths.max(initial=0))
     whole = longest * experts <= 4096
     size = max(1, longest) if whole else max(16, -(-tokens // (4 * num_cu)))
-    tiles = []
-    for g, (a, n) in enumerate(zip(offsets, lengths)):
-        parts = -(-n // size)
-        for q in range(parts):
-            tiles.append((a + n * q // parts, a + n * (q + 1) // parts, g, -1 if parts == 1 else q))
-    size = max(size, 16)
-    for a in range(offsets[-1], tokens, size):  # behind the last group
-        tiles.append((a, min(tokens, a + size), -1, 0))
-    return tiles, whole
+    parts = -(-lengths // size)
+    group = np.repeat(np.arange(len(lengths)), parts)
+    part = np.arange(len(group)) - np.repeat(np.cumsum(parts) - parts, parts)
+    begin = offsets[:-1][group] + lengths[group] * part // np.maximum(parts[group], 1)
+    end = offsets[:-1][group] + lengths[group] * (part + 1) // np.maximum(parts[group], 1)
+    part[parts[group] == 1] = -1
+    behind = np.arange(offsets[-1], tokens, max(size, 16))  # tokens behind the last group
+    tiles = np.stack([np.concatenate([begin, behind]), np.concatenate([end, np.minimum(behind + max(size, 16), tokens)]),
+                      np.concatenate([group, np.full(len(behind), -1)]), np.concatenate([part, np.zeros(len(behind), np.int64)])], axis=1)
+    return tiles, size, whole
 
 
 class BalanceLoss(_RowLoss):
@@ -337,17 +339,22 @@ class BalanceLoss(_RowLoss):
         self.ctx = _common_device((mask, chosen), ctx)
         dev = self.ctx.torch_device
         groups = len(offsets) - 1
-        tiles, whole = _balance_tiles(self.rows, self.classes, offsets, self.ctx.device_info()["compute_units"])
-        packed = np.array([(b, e, (g & 0xFFFFFFFF) | ((part & 0xFFFFFFFF) << 32)) for b, e, g, part in tiles], np.uint64).reshape(-1, 3).view(np.int64)
+        tiles, size, whole = _balance_tiles(self.rows, self.classes, offsets, self.ctx.device_info()["compute_units"])
+        even = offsets == [0, self.rows]  # one group: its tiles need no list
+        ntiles = -(-self.rows // size) if even else len(tiles)
+        last_part = ntiles - 1 if even else int(tiles[:, 3].max(initial=0))
+        packed = np.empty((len(tiles), 3), np.int64)  # pg_balance_tile: two int64, two int32
+        packed[:, :2] = tiles[:, :2]
+        packed[:, 2] = (tiles[:, 2] & 0xFFFFFFFF) | (tiles[:, 3] << 32)
         with _Ordered(self.ctx):
-            tiles_d = torch.from_numpy(packed).to(dev)
+            tiles_d = None if even else torch.from_numpy(packed).to(dev)
             mask, chosen = (None if v is None else v.to(dev) for v in (mask, chosen))
             self._counts = torch.zeros(groups, self.classes, dtype=torch.int32, device=dev)
-            copies = min(16, 1 + max((max(part, 0) for *_, part in tiles), default=0) // 16)  # some sixteen tiles to an accumulator
+            copies = min(16, 1 + max(last_part, 0) // 16)  # some sixteen tiles to an accumulator
             state = torch.zeros(4 + (0 if whole else 2 * groups * copies * (self.classes + 2)), dtype=torch.int32, device=dev)
         self._keep = tiles_d, mask, chosen, state
         ptr = lambda v: None if v is None else v.data_ptr()  # noqa: E731
-        self._b = _lib.pg_balance(tokens=self.rows, groups=groups, ntiles=len(tiles), tiles=ptr(tiles_d), mask=ptr(mask), chosen=ptr(chosen),
+        self._b = _lib.pg_balance(tokens=self.rows, groups=groups, ntiles=ntiles, tile_tokens=size, tiles=ptr(tiles_d), mask=ptr(mask), chosen=ptr(chosen),
                                   chosen_ld=0 if chosen is None else (chosen.stride(0) if self.rows > 1 else self.k), counts=ptr(self._counts),
                                   state=ptr(state), experts=self.classes, k=self.k,
                                   chosen_bits=64 if chosen is not None and chosen.dtype == torch.int64 else 32, whole=whole, copies=copies, lam=self.lam)

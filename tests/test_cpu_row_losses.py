@@ -88,11 +88,11 @@ def test_balance_tiles_cover_every_token_once():
     from proximalalgorithms.jl_amd.row_losses import _balance_tiles
 
     for tokens, offsets in ((0, [0, 0]), (1, [0, 1]), (5, [0, 0, 0, 4]), (1000, [0, 1, 1, 700, 999]), (100000, [0, 100000]), (4096, list(range(4097)))):
-        tiles, whole = _balance_tiles(tokens, 60, offsets, 256)
+        tiles, size, whole = _balance_tiles(tokens, 60, offsets, 256)
         seen = np.zeros(tokens, int)
         first = set()
         for b, e, g, part in tiles:
-            assert 0 <= b < e <= tokens and -1 <= g < len(offsets) - 1
+            assert 0 <= b < e <= tokens and -1 <= g < len(offsets) - 1 and e - b <= max(size, 16)
             seen[b:e] += 1
             if g >= 0:
                 assert offsets[g] <= b and e <= offsets[g + 1]
