@@ -35,6 +35,7 @@ struct DArgs {
   int64_t ldx, ldg, ldt, ldi, row0, nrows;  // rows of this launch
   int V, K, tdt, ibits, lsedt, wdt, labbits;
   double invT, lam, lab_lam;
+  int squares;  // T = 2: 1, T = 4: 2, else 0
   int parts, pv;  // parts of a row, 16-byte vectors per part
   double *stat, *xk;
   double *partials, *acc, *out;
@@ -123,13 +124,35 @@ __device__ __forceinline__ unsigned listed_bits(const unsigned* bm, int vbit) { 
   return (bm[vbit >> 5] >> (vbit & 31)) & ((1u << N) - 1u);
 }
 
+// what(i, exp(x_i - m)) for each i, beside e = exp((x - m) / T): e squared once for T = 2, twice for T = 4 (`squares`; a rounding each,
+// against a whole exponential), else an exponential of its own
+template <typename C, int N, typename F>
+__device__ __forceinline__ void power(int squares, const C (&x)[N], const C (&e)[N], C m, F what) {
+  if (squares == 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) what(i, e[i] * e[i]);
+  } else if (squares == 2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) what(i, (e[i] * e[i]) * (e[i] * e[i]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) what(i, ex2((x[i] - m) * (C)LOG2E));
+  }
+}
+// e, or 0 if bit i is set
+__device__ __forceinline__ float without(float e, unsigned bits, int i) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(int, e) & ~((int)(bits << (31 - i)) >> 31));
+}
+__device__ __forceinline__ double without(double e, unsigned bits, int i) { return (bits >> i) & 1u ? 0.0 : e; }
+
 // Sums of one thread, relative to a reference score m that is one of the row's (or the type's lowest value while there is
 // none): any score will do that is no more than 59 powers of two (41 = 59 ln 2) below the largest, so m is raised rarely, by a branch.
 template <typename C, bool TAIL, bool TWO>
 struct Run {
   C m = Lim<C>::lowest, lim = Lim<C>::lowest, s = C(0), sl = C(0), s1 = C(0), n = C(0);
   C c, head;  // log2(e) / T; 59 powers of two in scores
-  __device__ __forceinline__ explicit Run(double invT) : c(uniform((C)(invT * LOG2E))), head(uniform((C)(41.0 / fmax(invT, 1.0)))) {}
+  int squares;
+  __device__ __forceinline__ Run(double invT, int sq) : c(uniform((C)(invT * LOG2E))), head(uniform((C)(41.0 / fmax(invT, 1.0)))), squares(sq) {}
   __device__ __forceinline__ void raise(C to) {
     const C d = m - to;
     const C f = ex2(d * c);
@@ -155,19 +178,14 @@ struct Run {
 #pragma unroll
     for (int i = 0; i < N; ++i) e[i] = ex2((f[i] - m) * c);
     if constexpr (TWO) {
-      C t[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) t[i] = ex2((f[i] - m) * (C)LOG2E);
-#pragma unroll
-      for (int o = 1; o < N; o *= 2)
-#pragma unroll
-        for (int i = 0; i < N; i += 2 * o) t[i] += t[i + o];
-      s1 += t[0];
+      C t[2] = {C(0), C(0)};
+      power(squares, f, e, m, [&](int i, C v) { t[i & 1] += v; });
+      s1 += t[0] + t[1];
     }
     if constexpr (TAIL) {
       if (bits) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) e[i] = (bits >> i) & 1u ? C(0) : e[i];
+        for (int i = 0; i < N; ++i) e[i] = without(e[i], bits, i);
       }
     }
 #pragma unroll
@@ -232,7 +250,7 @@ __global__ __launch_bounds__(PT) void distill_part_stats(DArgs a) {
     for (int i = tid; i < q.words; i += PT) bm[i] = 0;
     __syncthreads();
   }
-  Run<C, TAIL, TWO> run(a.invT);
+  Run<C, TAIL, TWO> run(a.invT, a.squares);
   bool bad = false;
   for (int k = tid; k < a.K; k += PT) {
     const int64_t id = ld_int(a.idx, a.ibits, q.row * a.ldi + k);
@@ -638,26 +656,8 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     ask_list(nrow, id_raw, t_next, y_raw);
 
     // pass 1
-    Run<C, tail, two> run(a.invT);
-    int t0 = tid;
-    opaque(t0);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (j * NT < pl.nmain) {
-        if ((j + 1) * NT > pl.nmain) {
-          if (j * NT + t0 >= pl.nmain) d[j] = minus_inf16<T>();
-          opaque(d[j]);  // keep the branch: every vector but one is whole
-        }
-        C f[N];
-        unpack<T>(d[j], f);
-        run.template add<N>(f, tail ? listed_bits<T>(bm, min(j * NT + t0, pl.nmain) * N + BIT0) : 0u);
-      }
-    }
-    if (ee >= 0) {
-      const int b = ee - bbase;
-      run.add1(up<T>(edge), tail && ((bm[b >> 5] >> (b & 31)) & 1u));
-    }
-    // the list: the teacher's maximum and sum, the scores the sums have left out
+    Run<C, tail, two> run(a.invT, a.squares);
+    // the list, while the row is on its way: the teacher's maximum and sum, the scores that the sums below leave out
     C tm = Lim<C>::lowest, ts = C(0);
     double tmass = 0.0;
     bool bad = y == -2;
@@ -678,6 +678,24 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
         }
         ts += ex2((t - tm) * (C)LOG2E);
       }
+    }
+    int t0 = tid;
+    opaque(t0);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (j * NT < pl.nmain) {
+        if ((j + 1) * NT > pl.nmain) {
+          if (j * NT + t0 >= pl.nmain) d[j] = minus_inf16<T>();
+          opaque(d[j]);  // keep the branch: every vector but one is whole
+        }
+        C f[N];
+        unpack<T>(d[j], f);
+        run.template add<N>(f, tail ? listed_bits<T>(bm, min(j * NT + t0, pl.nmain) * N + BIT0) : 0u);
+      }
+    }
+    if (ee >= 0) {
+      const int b = ee - bbase;
+      run.add1(up<T>(edge), tail && ((bm[b >> 5] >> (b & 31)) & 1u));
     }
     if (bad) run.s = (C)NAN;
     // joined over the group
@@ -747,6 +765,11 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     int off = tid * 16;
     opaque(off);  // NV sums that stay out of the row loop's registers
     auto entry = [&](C x, C coef) { return ex2((x - rs.M) * c) * coef + (two ? ex2((x - rs.M) * (C)LOG2E) * rs.c1 : C(0)); };
+    // For the two-byte types the coefficient goes into the exponent, |cR| exp2((x - M) c) = exp2((x - M) c + log2 |cR|): an operation
+    // a score less.  The logarithm, 100 at most in earnest, is off by 2^-18: 3e-6 of an entry that is then rounded by up to
+    // 2^-12 (Float16) of it.
+    const C fold = uniform(lg2((C)fabs(rs.cR)));
+    const unsigned sign = rs.cR < C(0) ? 0x80008000u : 0u;  // (without an outside class cR is not negative)
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       // (stores and loads without a branch: what lies behind a row's end is dropped by the bounds check, and the compiler can
@@ -756,13 +779,22 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
       if (j * NT < pl.nmain) {
         C x[N], o[N];
         unpack<T>(d[j], x);
+        if constexpr (sizeof(T) == 2 && !two) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = ex2((x[i] - rs.M) * c) * rs.cR;
-        if constexpr (two) {
+          for (int i = 0; i < N; ++i) o[i] = ex2(fma(x[i] - rs.M, c, fold));
+          out = pack<T>(o);
+          if constexpr (tail) out ^= u32x4{sign, sign, sign, sign};
+        } else {
 #pragma unroll
-          for (int i = 0; i < N; ++i) o[i] += ex2((x[i] - rs.M) * (C)LOG2E) * rs.c1;
+          for (int i = 0; i < N; ++i) o[i] = ex2((x[i] - rs.M) * c);
+          if constexpr (two) {
+            power(a.squares, x, o, rs.M, [&](int i, C v) { o[i] = o[i] * rs.cR + v * rs.c1; });
+          } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) o[i] *= rs.cR;
+          }
+          out = pack<T>(o);
         }
-        out = pack<T>(o);
       }
       stb16(rg, off + j * NT * 16, out);
       d[j] = ldb16(rn, off + j * NT * 16);

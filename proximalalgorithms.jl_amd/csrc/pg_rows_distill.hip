@@ -54,6 +54,7 @@ pg_status pg_distill_value_and_gradient(pg_ctx* c, const pg_distill* d, int32_t 
     a.V = (int)d->classes, a.K = (int)d->top;
     a.tdt = d->teacher_dtype, a.ibits = d->index_bits, a.lsedt = d->lse_dtype, a.wdt = d->weights_dtype, a.labbits = d->label_bits;
     a.invT = 1.0 / d->temperature, a.lam = d->lam, a.lab_lam = d->label_lam;
+    a.squares = d->temperature == 2.0 ? 1 : (d->temperature == 4.0 ? 2 : 0);
     a.partials = c->red_partials, a.counter = c->row_tickets, a.out = out, a.value = value;
     PG_TRY(dtype == PG_F32 ? distill_f32(c, a, d->rows) : dtype == PG_F64 ? distill_f64(c, a, d->rows)
            : dtype == PG_BF16 ? distill_bf16(c, a, d->rows) : distill_f16(c, a, d->rows));
