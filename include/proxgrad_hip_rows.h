@@ -9,7 +9,7 @@
  *
  * Element types: scores and gradients are PG_F32, PG_F64, PG_BF16 or PG_F16.  Arithmetic, softmax statistics and sums are
  * Float32 for the three narrow types and Float64 for PG_F64; the total over the rows is Float64; each gradient entry is
- * rounded to the scores' type once.
+ * rounded to the scores' type once.  In Float32 a probability of less than 2^-126 of the row's largest is 0.
  *
  * Rows are `ld` elements apart (ld >= the row's length), elements of a row are adjacent, no alignment is asked for beyond
  * the element's own.  What lies between the rows is neither read nor written.  grad may be the scores' own buffer (same
@@ -47,7 +47,7 @@ enum { PG_BF16 = 2, PG_F16 = 3 }; /* beside PG_F32, PG_F64: understood by this h
  * and leaves the gradient finite.  A NaN among a row's scores, or an index or label outside [-1, classes), makes f and that
  * row's gradient NaN. */
 typedef struct pg_distill {
-  int64_t rows, classes, top; /* classes < 2^30, top <= 1024 */
+  int64_t rows, classes, top; /* classes <= 2^24, top <= 1024 */
   const void* teacher;        /* [rows x top], any element type; may be NULL with top = 0 */
   int64_t teacher_ld;
   const void* index; /* [rows x top], int32 or int64 */

@@ -48,13 +48,18 @@ def distillation(x, t, idx, *, temperature=1.0, lam=1.0, teacher_lse=None, weigh
         np.add.at(phat, cls, p)
         with np.errstate(invalid="ignore"):
             np.add.at(ksize, cls, np.where(p > 0, p * (64 + 4 * np.abs(lp)), 0.0))
-        pr, rest = L(0), np.zeros(v, L)
+        pr, rest, left_size = L(0), np.zeros(v, L), L(0)
         outside = np.ones(v, bool)
         outside[cls] = False
         if teacher_lse is not None and len(tt) and outside.any():
             pr = max(L(0), L(1) - p.sum())
             qr = q[outside].sum()
             rest[outside] = pr / qr if qr > 0 else 0.0
+            # 1 - sum p is as far off as the sum is, (64 + 4 |log p|) roundings of each p, however little is left; an entry outside
+            # the list gets q / Q of that, the value its slope log pr - log Q + 1 times that
+            left_size = (p[p > 0] * (64 + 4 * np.abs(lp[p > 0]))).sum()
+            if qr > 0:
+                ksize[outside] += left_size * q[outside] / qr
         elif teacher_lse is not None and len(tt) == 0:
             pr, qr, rest = L(1), L(1), np.ones(v, L)  # nothing listed: the outside class is everything on both sides
         mass = p.sum() + pr
@@ -63,6 +68,7 @@ def distillation(x, t, idx, *, temperature=1.0, lam=1.0, teacher_lse=None, weigh
             sizes = np.where(p > 0, p * (64 + 8 * (np.abs(lp) + np.abs(lq[cls]) + np.abs(x[i][cls]) / temperature)), 0.0)
             row = terms.sum() + (pr * (np.log(pr) - np.log(qr)) if pr > 0 else 0.0)
             row_size = sizes[np.isfinite(sizes)].sum() + (64 * pr * (1 + abs(np.log(pr)) + abs(np.log(qr))) + 64 * (1 + abs(np.log(qr))) if pr > 0 and qr > 0 else 0.0)
+            row_size += left_size * (1 + abs(np.log(pr)) + abs(np.log(qr))) if pr > 0 and qr > 0 and left_size else 0.0
         f += lam * w * row
         f_size += lam * w * row_size
         grad[i] = lam * w / temperature * (mass * q - phat - rest * q)

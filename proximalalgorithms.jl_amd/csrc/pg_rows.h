@@ -90,7 +90,7 @@ template <typename T>
 __device__ __forceinline__ void st16(T* p, u32x4 v) {
   reinterpret_cast<Loose<T>*>(p)->v = v;
 }
-// vector v of a row: a wave-uniform base and a 32-bit offset (a row is at most 2^30 elements of at most 8 bytes: the product is unsigned)
+// vector v of a row: a wave-uniform base and a 32-bit offset (a row is at most 2^24 elements of at most 8 bytes)
 template <typename T>
 __device__ __forceinline__ T* at16(T* base, int v) {
   return (T*)((const char*)base + (uint64_t)(unsigned)v * 16u);  // (through char*: an integer would lose the address space)
@@ -188,6 +188,7 @@ __device__ __forceinline__ int64_t ld_int_u(const void* p, int bits, int64_t i) 
 __device__ __forceinline__ float uniform(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))); }
 __device__ __forceinline__ double uniform(double v) { return pg_readlane(v, 0); }
 
+// (one instruction; results below 2^-126 are 0)
 __device__ __forceinline__ float ex2(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ double ex2(double v) { return exp2(v); }
 __device__ __forceinline__ float lg2(float v) { return __builtin_amdgcn_logf(v); }

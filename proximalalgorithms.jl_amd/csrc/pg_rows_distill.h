@@ -27,6 +27,8 @@ constexpr int BIT0 = 8;         // bits in front of a chunk's first aligned vect
 constexpr int STAT = 6;         // doubles per (row, part)
 constexpr int MAX_PARTS = 64;   // one lane each when a row's parts are joined
 constexpr int MAX_TOP = 1024;
+constexpr int PART_BITS = 32 * 1024 * 8;                          // classes of a part: its bitmap takes 32 KiB of LDS
+constexpr int64_t MAX_CLASSES = (int64_t)MAX_PARTS * PART_BITS;  // 2^24
 
 struct DArgs {
   const void* x;
@@ -146,13 +148,14 @@ __device__ __forceinline__ float without(float e, unsigned bits, int i) {
 __device__ __forceinline__ double without(double e, unsigned bits, int i) { return (bits >> i) & 1u ? 0.0 : e; }
 
 // Sums of one thread, relative to a reference score m that is one of the row's (or the type's lowest value while there is
-// none): any score will do that is no more than 59 powers of two (41 = 59 ln 2) below the largest, so m is raised rarely, by a branch.
+// none): any score will do that is not far below the largest, so m is raised rarely, by a branch.  Far:
+// an exponent of 20, whose rounding is 20 * 2^-24 of its exponential, like those of the terms that count least.
 template <typename C, bool TAIL, bool TWO>
 struct Run {
   C m = Lim<C>::lowest, lim = Lim<C>::lowest, s = C(0), sl = C(0), s1 = C(0), n = C(0);
-  C c, head;  // log2(e) / T; 59 powers of two in scores
+  C c, head;  // log2(e) / T; an exponent of 20 in scores
   int squares;
-  __device__ __forceinline__ Run(double invT, int sq) : c(uniform((C)(invT * LOG2E))), head(uniform((C)(41.0 / fmax(invT, 1.0)))), squares(sq) {}
+  __device__ __forceinline__ Run(double invT, int sq) : c(uniform((C)(invT * LOG2E))), head(uniform((C)(20.0 / fmax(invT, 1.0)))), squares(sq) {}
   __device__ __forceinline__ void raise(C to) {
     const C d = m - to;
     const C f = ex2(d * c);
@@ -461,7 +464,7 @@ pg_status run_parts(pg_ctx* c, DArgs a, int64_t rows) {
   constexpr int N = Elem<T>::N;
   const int64_t vecs = (a.V + N - 1) / N;
   // two workgroups per CU if the rows are few, but no part below 2 vectors a thread, and none that its bitmap does not hold
-  const int64_t most = (32 * 1024 * 8) / N;
+  const int64_t most = PART_BITS / N;
   int64_t parts = (2 * c->num_cu + rows - 1) / rows;
   parts = std::min<int64_t>(parts, (vecs + 2 * PT - 1) / (2 * PT));
   parts = std::max<int64_t>(parts, (vecs + most - 1) / most);
@@ -469,10 +472,6 @@ pg_status run_parts(pg_ctx* c, DArgs a, int64_t rows) {
   a.parts = (int)parts;
   a.pv = (int)((vecs + parts - 1) / parts);
   const size_t lds = ((size_t)a.pv * N + BIT0 + N + 31) / 32 * 4 + 4;
-  if (lds > 62 * 1024) {
-    pg_set_error("pg_distill: rows of more than %lld classes are not supported", (long long)MAX_PARTS * 62 * 1024 * 8);
-    return PG_ERR_UNSUPPORTED;
-  }
   const int64_t ws = (int64_t)PG_RED_MAX_BLOCKS * (PG_RED_MAX_NS - 1) - 8;  // doubles behind the reduction's own partials
   const int64_t batch = std::min<int64_t>(ws / (parts * STAT + a.K + 1), PG_RED_MAX_BLOCKS);
   a.acc = c->red_partials + PG_RED_MAX_BLOCKS;

@@ -21,7 +21,7 @@ pg_status pg_distill_value_and_gradient(pg_ctx* c, const pg_distill* d, int32_t 
   PG_REQUIRE(c != nullptr && d != nullptr, "null argument");
   PG_REQUIRE(dtype_ok(dtype), "bad dtype");
   PG_REQUIRE(d->rows >= 0 && d->classes >= 0 && d->top >= 0, "negative size");
-  PG_REQUIRE(d->classes < (1ll << 30), "classes must be below 2^30");
+  PG_REQUIRE(d->classes <= MAX_CLASSES, "at most 2^24 classes");
   PG_REQUIRE(d->top <= MAX_TOP, "top must be at most 1024");
   PG_REQUIRE(d->temperature > 0.0 && std::isfinite(d->temperature), "temperature must be positive and finite");
   PG_REQUIRE(d->lam >= 0.0 && d->label_lam >= 0.0 && std::isfinite(d->lam) && std::isfinite(d->label_lam), "lam and label_lam must be nonnegative and finite");

@@ -477,7 +477,8 @@ class IndAffine:
 
 class SlicedSeparableSum:
     """ProximalOperators.SlicedSeparableSum for contiguous ranges: h(y) = sum_k h_k(y[lo_k:hi_k]); the prox acts on
-    device views of the slices (0-based half-open ranges; element offsets must keep 16-byte alignment)."""
+    device views of the slices (0-based half-open ranges; element offsets must keep 16-byte alignment).  Of smooth terms it is
+    a smooth term itself: value_and_gradient writes each term's gradient into its slice."""
 
     def __init__(self, fs, ranges):
         self.fs, self.ranges = tuple(fs), tuple((int(lo), int(hi)) for lo, hi in ranges)
@@ -494,6 +495,41 @@ class SlicedSeparableSum:
         for f, (lo, hi) in zip(self.fs, self.ranges):
             total = R(total + f.prox_(self._view(y, lo, hi), self._view(x, lo, hi), gamma))
         return total
+
+    def value_and_gradient(self, x, out=None):
+        """(f(x), grad f(x)) for smooth terms: sum_k f_k(x[lo_k:hi_k]); zero where no range reaches.  Ranges may not overlap."""
+        at = 0
+        gaps = False
+        for lo, hi in sorted(self.ranges):
+            if not (at <= lo <= hi <= x.n):
+                raise ValueError(f"ranges of smooth terms must not overlap and must lie within the vector's {x.n} elements")
+            gaps |= lo > at
+            at = hi
+        g = out if out is not None else x.similar()
+        if gaps or at < x.n:
+            if g.ptr == x.ptr:
+                raise ValueError("ranges that leave out a part of x need a gradient apart from x")
+            g.fill_(0.0)
+        total = 0.0
+        for f, (lo, hi) in zip(self.fs, self.ranges):
+            if lo < hi:
+                total += float(value_and_gradient_(self._view(g, lo, hi), f, self._view(x, lo, hi)))
+        return x.dtype.type(total), g
+
+    def __call__(self, x):
+        total = 0.0
+        for f, (lo, hi) in zip(self.fs, self.ranges):
+            if lo < hi:
+                total += float(f(self._view(x, lo, hi)))
+        return x.dtype.type(total)
+
+    @property
+    def is_convex(self):
+        return all(getattr(f, "is_convex", False) for f in self.fs)
+
+    @property
+    def is_generalized_quadratic(self):
+        return all(getattr(f, "is_generalized_quadratic", False) for f in self.fs)
 
 
 class IndZero:

@@ -80,6 +80,22 @@ def _raw_stream(device):
     return fast(device) if fast is not None else torch.cuda.current_stream(device).cuda_stream
 
 
+def _stream_of(ctx):
+    torch = _torch()
+    return torch.cuda.ExternalStream(ctx.stream, device=ctx.torch_device) if ctx.stream else torch.cuda.default_stream(ctx.torch_device)
+
+
+def _settle(ctx, tensors):
+    """a new loss's tensors: what the current stream still does to them comes before the context's later work, and their memory
+    is not handed out again while the context uses it"""
+    with _Ordered(ctx):
+        pass
+    if _raw_stream(ctx.device) != ctx.stream:
+        for v in tensors:
+            if v is not None and v.numel():
+                v.record_stream(_stream_of(ctx))
+
+
 class _Ordered:
     """the call's kernels run on the context's stream: between the current torch stream's past and its future"""
 
@@ -100,7 +116,7 @@ class _Ordered:
                 if torch.cuda.is_current_stream_capturing():
                     raise ProxGradError("a torch graph is being recorded: record with Context.capture_begin instead",
                                         code=_lib.PG_ERR_UNSUPPORTED)
-                self.cur, self.ext = cur, torch.cuda.ExternalStream(ctx.stream, device=ctx.torch_device)
+                self.cur, self.ext = cur, _stream_of(ctx)
                 self.ext.wait_stream(cur)
 
     def __exit__(self, *exc):
@@ -114,6 +130,12 @@ class _RowLoss:
 
     is_generalized_quadratic = False
 
+    def _open(self, ctx, *tensors):
+        self.ctx = _common_device(tensors, ctx)
+        if self.ctx.capturing:
+            raise ProxGradError("device allocation during stream capture: make the loss before")
+        return self.ctx.torch_device
+
     def _locate(self, u, name):
         """(pointer, row distance, dtype code) of scores or gradients"""
         n, v = self.rows, self.classes
@@ -122,6 +144,8 @@ class _RowLoss:
                 raise ValueError(f"{name} must hold {n} x {v} scores, got {u.n}")
             if u.ctx.device != self.ctx.device:
                 raise ValueError(f"{name} lives on another device than the loss")
+            if u.ctx.stream != self.ctx.stream:
+                raise ValueError(f"{name} belongs to a context on another stream than the loss's")
             return u.ptr, max(v, 1), u.pg_dtype
         code = _dtype_code(getattr(u, "dtype", None))
         if code is None:
@@ -209,7 +233,8 @@ class DistillationLoss(_RowLoss):
     p is the softmax of the listed logits / T; with ``teacher_lse`` -- log sum exp of ALL the teacher's logits / T per row -- it is the
     teacher's own probability, and the classes outside the list count as one more class (then f is not convex).  ``labels``: -1 = none.
     The usual factor T^2 is the caller's: ``lam=T**2``.  Rows of weight 0 are not read.  Tensors on the device are used where
-    they are, later changes included; host arrays are checked and uploaded.  An index or label that is out of range on the
+    they are, later changes included (a copy of those whose last axis is not dense or whose type is none of Float32, Float64 --
+    logits bfloat16 and Float16 too --, int32, int64); host arrays are checked and uploaded.  An index or label that is out of range on the
     device makes the value and that row's gradient NaN."""
 
     def __init__(self, teacher_logits, teacher_index, n_classes, *, temperature=1.0, lam=1.0, teacher_lse=None, weights=None,
@@ -220,8 +245,8 @@ class DistillationLoss(_RowLoss):
             raise ValueError("teacher_logits must be a (rows, top) array")
         self.rows, top = int(t.shape[0]), int(t.shape[1])
         self.classes = int(n_classes)
-        if self.classes < 0 or self.classes >= 1 << 30:
-            raise ValueError("n_classes must be between 0 and 2^30 - 1")
+        if not 0 <= self.classes <= 1 << 24:
+            raise ValueError("n_classes must be between 0 and 2^24")
         if top > 1024:
             raise ValueError("at most 1024 listed logits per row")
         self.temperature, self.lam, self.label_lam = float(temperature), float(lam), float(label_lam)
@@ -243,9 +268,9 @@ class DistillationLoss(_RowLoss):
         if weights is not None and not weights.is_cuda and weights.numel() and not bool((weights >= 0).all()):
             raise ValueError("weights must be nonnegative")
         self.is_convex = lse is None
-        self.ctx = _common_device((t, index, lse, weights, labels), ctx)
-        dev = self.ctx.torch_device
+        dev = self._open(ctx, t, index, lse, weights, labels)
         self._keep = t, index, lse, weights, labels = [None if v is None else v.to(dev) for v in (t, index, lse, weights, labels)]
+        _settle(self.ctx, self._keep)
         ptr = lambda v: None if v is None else v.data_ptr()  # noqa: E731
         bits = lambda v: 64 if v is not None and v.dtype == torch.int64 else 32  # noqa: E731
         code = lambda v: PG_F32 if v is None else _dtype_code(v.dtype)  # noqa: E731
@@ -336,8 +361,7 @@ class BalanceLoss(_RowLoss):
             chosen = _rows_of(chosen, "chosen", (self.rows, self.k), (torch.int32, torch.int64), torch.int64)
             if not chosen.is_cuda and chosen.numel() and not (int(chosen.min()) >= -1 and int(chosen.max()) < self.classes):
                 raise ValueError("chosen must lie between -1 and n_experts - 1")
-        self.ctx = _common_device((mask, chosen), ctx)
-        dev = self.ctx.torch_device
+        dev = self._open(ctx, mask, chosen)
         groups = len(offsets) - 1
         tiles, size, whole = _balance_tiles(self.rows, self.classes, offsets, self.ctx.device_info()["compute_units"])
         even = offsets == [0, self.rows]  # one group: its tiles need no list
@@ -346,13 +370,13 @@ class BalanceLoss(_RowLoss):
         packed = np.empty((len(tiles), 3), np.int64)  # pg_balance_tile: two int64, two int32
         packed[:, :2] = tiles[:, :2]
         packed[:, 2] = (tiles[:, 2] & 0xFFFFFFFF) | (tiles[:, 3] << 32)
-        with _Ordered(self.ctx):
-            tiles_d = None if even else torch.from_numpy(packed).to(dev)
-            mask, chosen = (None if v is None else v.to(dev) for v in (mask, chosen))
-            self._counts = torch.zeros(groups, self.classes, dtype=torch.int32, device=dev)
-            copies = min(16, 1 + max(last_part, 0) // 16)  # some sixteen tiles to an accumulator
-            state = torch.zeros(4 + (0 if whole else 2 * groups * copies * (self.classes + 2)), dtype=torch.int32, device=dev)
+        tiles_d = None if even else torch.from_numpy(packed).to(dev)
+        mask, chosen = (None if v is None else v.to(dev) for v in (mask, chosen))
+        self._counts = torch.zeros(groups, self.classes, dtype=torch.int32, device=dev)
+        copies = min(16, 1 + max(last_part, 0) // 16)  # some sixteen tiles to an accumulator
+        state = torch.zeros(4 + (0 if whole else 2 * groups * copies * (self.classes + 2)), dtype=torch.int32, device=dev)
         self._keep = tiles_d, mask, chosen, state
+        _settle(self.ctx, (*self._keep, self._counts))
         ptr = lambda v: None if v is None else v.data_ptr()  # noqa: E731
         self._b = _lib.pg_balance(tokens=self.rows, groups=groups, ntiles=ntiles, tile_tokens=size, tiles=ptr(tiles_d), mask=ptr(mask), chosen=ptr(chosen),
                                   chosen_ld=0 if chosen is None else (chosen.stride(0) if self.rows > 1 else self.k), counts=ptr(self._counts),

@@ -47,7 +47,7 @@ def test_distillation_refusals():
     t, i = np.zeros((3, 2), np.float32), np.zeros((3, 2), np.int64)
     bad = [
         (ValueError, (t[0], i, 5), {}), (ValueError, (t, i[:2], 5), {}), (ValueError, (t, i + 5, 5), {}), (ValueError, (t, i - 2, 5), {}),
-        (ValueError, (t, i, -1), {}), (ValueError, (t, i, 1 << 30), {}), (TypeError, (t, t, 5), {}), (TypeError, (i, i, 5), {}),
+        (ValueError, (t, i, -1), {}), (ValueError, (t, i, (1 << 24) + 1), {}), (TypeError, (t, t, 5), {}), (TypeError, (i, i, 5), {}),
         (ValueError, (np.zeros((1, 1025), np.float32), np.zeros((1, 1025), int), 2000), {}),
         (ValueError, (t, i, 5), dict(temperature=0.0)), (ValueError, (t, i, 5), dict(temperature=float("inf"))),
         (ValueError, (t, i, 5), dict(lam=-1.0)), (ValueError, (t, i, 5), dict(lam=float("nan"))), (ValueError, (t, i, 5), dict(label_lam=1.0)),
@@ -151,3 +151,36 @@ def test_oracle_balance_gradient_is_its_differences():
             fp, fm = ref.balance(rp, 2, **kw), ref.balance(rm, 2, **kw)
             assert np.array_equal(fp[2], counts) and np.array_equal(fm[2], counts)  # no choice changes within h
             assert abs((fp[0] - fm[0]) / (2 * h) - g[i, j]) < 1e-8
+
+
+def test_entry_points_refuse_bad_plans_before_any_device_work():
+    """every check of the C entry points that needs no device; the context is a block of zeros that none of them may look into"""
+    from proximalalgorithms.jl_amd import _lib
+
+    lib = _lib.load()
+    ctx, mem = C.create_string_buffer(1 << 16), C.create_string_buffer(4096)
+    base, p = C.addressof(mem), C.cast(ctx, C.c_void_p)
+    good = dict(rows=2, classes=8, top=2, teacher=base, teacher_ld=2, index=base, index_ld=2, index_bits=32, temperature=1.0, lam=1.0)
+    for change, dtype, ld, shift in ((dict(rows=-1), 0, 8, 0), (dict(top=1025), 0, 8, 0), (dict(classes=(1 << 24) + 1), 0, 8, 0), (dict(temperature=0.0), 0, 8, 0),
+                                     (dict(temperature=float("nan")), 0, 8, 0), (dict(lam=-1.0), 0, 8, 0), (dict(label_lam=float("inf")), 0, 8, 0), (dict(teacher=None), 0, 8, 0),
+                                     (dict(teacher_dtype=7), 0, 8, 0), (dict(index_bits=16), 0, 8, 0), (dict(teacher_lse=base, lse_dtype=2), 0, 8, 0),
+                                     (dict(weights=base, weights_dtype=3), 0, 8, 0), (dict(labels=base, label_bits=8), 0, 8, 0), ({}, 4, 8, 0), ({}, 0, 7, 0), ({}, 0, 8, 2)):
+        d = _lib.pg_distill(**{**good, **change})
+        assert lib.pg_distill_value_and_gradient(p, C.byref(d), dtype, base + 64 + shift, ld, base + 2048, ld, None, None) == _lib.PG_ERR_INVALID, change
+    good = dict(tokens=2, groups=1, ntiles=1, tile_tokens=2, counts=base, state=base, experts=8, k=2, copies=1, lam=1.0)
+    for change, dtype, ld, shift in ((dict(tokens=-1), 0, 8, 0), (dict(tokens=1 << 31), 0, 8, 0), (dict(experts=0), 0, 8, 0), (dict(experts=1025), 0, 8, 0), (dict(k=9), 0, 8, 0),
+                                     (dict(k=0), 0, 8, 0), (dict(lam=float("nan")), 0, 8, 0), (dict(ntiles=2), 0, 8, 0), (dict(groups=2), 0, 8, 0), (dict(state=None), 0, 8, 0),
+                                     (dict(copies=0), 0, 8, 0), (dict(copies=17), 0, 8, 0), (dict(chosen=base, chosen_bits=16), 0, 8, 0), ({}, -1, 8, 0), ({}, 0, 7, 0), ({}, 0, 8, 1)):
+        b = _lib.pg_balance(**{**good, **change})
+        assert lib.pg_balance_value_and_gradient(p, C.byref(b), dtype, base + 64 + shift, ld, base + 2048, ld, None, None) == _lib.PG_ERR_INVALID, change
+
+
+def test_sum_of_smooth_terms_checks_its_ranges():
+    import proximalalgorithms.jl_amd as pa
+
+    x = pa.HIPVector(None, 1024, 100, np.float32)
+    for ranges in (((0, 60), (48, 100)), ((0, 101),), ((-4, 8),), ((16, 8),), ((0, 20), (0, 20))):
+        with pytest.raises(ValueError):
+            pa.SlicedSeparableSum((pa.SqrNormL2(),) * len(ranges), ranges).value_and_gradient(x)
+    assert pa.SlicedSeparableSum((pa.SqrNormL2(), pa.Zero()), ((0, 1), (4, 8))).is_convex
+    assert not pa.SlicedSeparableSum((pa.SqrNormL2(), object()), ((0, 1), (4, 8))).is_convex

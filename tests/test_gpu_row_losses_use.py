@@ -1,0 +1,401 @@
+"""The losses on rows of scores as they are used: every kernel form at full width, other layouts and types, streams, graphs, refusals,
+and both together as terms of one objective under the package's iterations.  Oracle and tolerances: test_gpu_row_losses.py."""
+import itertools
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import proxgrad_oracle as o
+from oracle import row_losses as ref
+from .test_gpu_row_losses import DT, check, check_balance, flushed, pa, router, scores, tdev, teacher
+
+pytestmark = pytest.mark.gpu
+SIZE = {"f32": 4, "f64": 8, "bf16": 2, "f16": 2}
+
+
+def repeated(n, base):
+    """rows 0 .. n - 1 are the distinct rows 0 .. base - 1 over and over: many rows, few for the oracle"""
+    return torch.arange(n, device="cuda") % base
+
+
+def check_repeated(g, val, want, dtype, n):
+    """each copy of a row against that row's gradient; the value is the rows' sum"""
+    f, grad, size, f_size = want[0]
+    base = grad.shape[0]
+    u = 2.0**-53 if dtype == torch.float64 else 2.0**-24
+    fin = torch.finfo(dtype)
+    for b in range(base):
+        tol = torch.from_numpy(np.abs(grad[b]) * (fin.eps / 2) + size[b] * u * 1.01 + fin.smallest_normal * fin.eps / 2).cuda()
+        if dtype != torch.float64:
+            tol += flushed(size[b:b + 1]).item()
+        off = (g[b::base].double() - torch.from_numpy(grad[b]).cuda()).abs_()
+        assert bool((off <= tol).all()), b
+    total = sum(w[0] * len(range(b, n, base)) for b, w in enumerate(want[1]))
+    slack = sum(w[3] * len(range(b, n, base)) for b, w in enumerate(want[1]))
+    assert abs(val - total) <= slack * u + abs(total) * (2.0**-24 if u > 1e-10 else 4 * u)
+
+
+# bytes of a row that each form holds, one class short of full (an odd number: rows at every alignment); 300 rows for the smaller
+# forms and 1100 for the larger, so that workgroups go on to further rows; the last one is longer than the registers
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("rest,labelled", [(False, False), (False, True), (True, False), (True, True)])
+@pytest.mark.parametrize("held,n", [(1024, 9000), (2048, 9000), (4096, 9000), (8192, 9000), (16384, 3000), (32768, 3000), (65536, 1100), (131072, 600),
+                                    (262144, 300), (280000, 70)])
+def test_every_form_at_full_width(dtype, rest, labelled, held, n):
+    v = held // SIZE[dtype] - 1
+    base, k, temperature = 3, 37, 2.0 if held % 3 else 1.25
+    rng = np.random.default_rng(held + 2 * rest + labelled)
+    t, idx = teacher(rng, base, v, k, twice=True)
+    td, te = tdev(t, torch.float32 if dtype != "f64" else torch.float64)
+    x, xe = scores(rng, base, v, DT[dtype], idx, t)
+    y = rng.integers(0, v, base)
+    y[1] = idx[1, 0]
+    kw = dict(temperature=temperature, lam=1.25)
+    lse = np.log(np.exp(te / temperature).sum(1) + 0.4) if rest else None
+    lse = None if lse is None else torch.from_numpy(lse).to(td.dtype)
+    each = repeated(n, base)
+    dev = dict(kw, teacher_lse=None if lse is None else lse.cuda()[each])
+    host = dict(kw, teacher_lse=None if lse is None else lse.double().numpy())
+    if labelled:
+        dev.update(labels=torch.from_numpy(y).cuda()[each], label_lam=0.5)
+        host.update(labels=y, label_lam=0.5)
+    f = pa().DistillationLoss(td[each], torch.from_numpy(idx).cuda()[each], v, **dev)
+    u = x[each]
+    val, g = f.value_and_gradient(u)
+    one = lambda b: {q: (w[b:b + 1] if isinstance(w, np.ndarray) else w) for q, w in host.items()}  # noqa: E731
+    alone = [ref.distillation(xe[b:b + 1], te[b:b + 1], idx[b:b + 1], **one(b)) for b in range(base)]
+    want = (None, np.concatenate([w[1] for w in alone]), np.concatenate([w[2] for w in alone]), None)
+    check_repeated(g, val, (want, alone), DT[dtype], n)
+    v2, _ = f.value_and_gradient_async(u, out=u)
+    assert torch.equal(u, g) and float(v2) == pytest.approx(val, rel=2.0**-23)  # in place, and the same again
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("temperature", [0.5, 1.0, 4.0])
+@pytest.mark.parametrize("n,v", [(5, 700), (5, 9001), (70, 40001)])
+def test_rising_scores(dtype, temperature, n, v):
+    """every score above the ones before it, over a wide range: the sums' reference is raised again and again"""
+    rng = np.random.default_rng(v)
+    t, idx = teacher(rng, n, v, 6)
+    xe = np.linspace(-300, 11, v) * np.linspace(0.1, 1, n)[:, None]
+    xd = torch.from_numpy(xe).to(DT[dtype]).cuda()
+    td, te = tdev(t, torch.float32)
+    lse = torch.from_numpy(np.log(np.exp(te / temperature).sum(1) * 1.5)).float()
+    y = rng.integers(0, v, n)
+    kw = dict(temperature=temperature, label_lam=0.5)
+    f = pa().DistillationLoss(td, torch.from_numpy(idx).cuda(), v, teacher_lse=lse.cuda(), labels=torch.from_numpy(y).cuda(), **kw)
+    val, g = f.value_and_gradient(xd)
+    rows = sorted({0, 1, n // 2, n - 1})
+    want = ref.distillation(xd.double().cpu().numpy()[rows], te[rows], idx[rows], teacher_lse=lse.double().numpy()[rows], labels=y[rows], **kw)
+    w = torch.zeros(n)
+    w[rows] = 1.0
+    f = pa().DistillationLoss(td, torch.from_numpy(idx).cuda(), v, teacher_lse=lse.cuda(), labels=torch.from_numpy(y).cuda(), weights=w.cuda(), **kw)
+    val, g1 = f.value_and_gradient(xd)
+    check(g1[rows], val, want, DT[dtype])
+    assert torch.equal(g1[rows], g[rows]) and not g1[[i for i in range(n) if i not in rows]].any()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("n,v,k", [(3, 1100, 1024), (70, 1024, 1024), (66, 20000, 700), (2, 90001, 1024), (3, 50, 0)])
+def test_long_and_empty_lists(dtype, rest, n, v, k):
+    rng = np.random.default_rng(k + n)
+    t, idx = teacher(rng, n, v, k, absent=0.1 if k < v else 0.0, twice=k < v)
+    td, te = tdev(t, DT[dtype])
+    x, xe = scores(rng, n, v, DT[dtype], idx, t)
+    with np.errstate(divide="ignore"):
+        lse = np.log(np.where(idx >= 0, np.exp(te), 0).sum(1) + 1e-3)
+    lse = torch.from_numpy(lse).float() if rest else None
+    w = np.zeros(n)
+    rows = sorted({0, n // 3, n - 1})
+    w[rows] = 1.5
+    f = pa().DistillationLoss(td, torch.from_numpy(idx).cuda(), v, weights=torch.from_numpy(w).cuda(), teacher_lse=None if lse is None else lse.cuda())
+    val, g = f.value_and_gradient(x)
+    check(g, val, ref.distillation(xe, te, idx, weights=w, teacher_lse=None if lse is None else lse.double().numpy()), DT[dtype])
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("logits", DT)
+@pytest.mark.parametrize("n,v", [(9, 301), (2, 40000)])
+def test_types_and_strides_of_the_teacher(dtype, logits, n, v):
+    """logits of each type beside scores of each type; lists that are columns of a wider table; Float64 weights and lse; int32, int64"""
+    rng = np.random.default_rng(7)
+    k = 11
+    t, idx = teacher(rng, n, v, k)
+    wide = torch.full((n, k + 5), float("nan"), dtype=DT[logits], device="cuda")
+    wide[:, 2:2 + k] = torch.from_numpy(t).to(DT[logits]).cuda()
+    te = wide[:, 2:2 + k].double().cpu().numpy()
+    wide_i = torch.full((n, k + 3), -7, dtype=torch.int32 if n > 2 else torch.int64, device="cuda")
+    wide_i[:, 3:] = torch.from_numpy(idx).cuda()
+    x, xe = scores(rng, n, v, DT[dtype], idx, t)
+    w = rng.random(n)
+    lse = np.log(np.exp(te).sum(1) * 1.25)
+    y = torch.from_numpy(rng.integers(-1, v, n)).to(torch.int32)
+    f = pa().DistillationLoss(wide[:, 2:2 + k], wide_i[:, 3:], v, teacher_lse=torch.from_numpy(lse).cuda(), weights=torch.from_numpy(w).cuda(),
+                              labels=y.cuda(), label_lam=0.25)
+    val, g = f.value_and_gradient(x)
+    check(g, val, ref.distillation(xe, te, idx, teacher_lse=lse, weights=w, labels=y.numpy(), label_lam=0.25), DT[dtype])
+    transposed = torch.from_numpy(np.ascontiguousarray(idx.T)).cuda().t()  # not dense along the list: copied
+    f = pa().DistillationLoss(te.astype(np.float64), transposed, v, teacher_lse=lse, weights=w, labels=y.numpy(), label_lam=0.25)  # and from the host
+    v2, g2 = f.value_and_gradient(x)
+    check(g2, v2, ref.distillation(xe, te, idx, teacher_lse=lse, weights=w, labels=y.numpy(), label_lam=0.25), DT[dtype])
+
+
+def both_losses(n=40, v=333, e=61, dt=torch.float32, ctx=None, seed=0):
+    rng = np.random.default_rng(seed)
+    t, idx = teacher(rng, n, v, 9)
+    d = pa().DistillationLoss(t, idx, v, temperature=2.0, labels=rng.integers(0, v, n), label_lam=0.5, ctx=ctx)
+    b = pa().BalanceLoss(n, e, 4, offsets=[0, n // 2, n - 1], ctx=ctx)
+    gen = torch.Generator("cuda").manual_seed(seed)
+    return (d, torch.randn(n, v, device="cuda", generator=gen).to(dt)), (b, torch.randn(n, e, device="cuda", generator=gen).to(dt))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("gap,shift", [(0, 1), (3, 0), (8, 5)])
+def test_out_of_another_layout_and_what_lies_between_the_rows(dtype, which, gap, shift):
+    loss, u = both_losses(dt=DT[dtype])[which]
+    n, v = u.shape
+    val, g = loss.value_and_gradient(u)
+    buf = torch.full((shift + n * (v + gap) + 9,), 7.0, dtype=u.dtype, device="cuda")
+    out = buf[shift:shift + n * (v + gap)].view(n, v + gap)[:, :v]
+    v2, g2 = loss.value_and_gradient(u, out=out)
+    assert g2 is out and torch.equal(out, g) and v2 == val
+    keep = torch.ones_like(buf, dtype=torch.bool)
+    keep[shift:shift + n * (v + gap)].view(n, v + gap)[:, :v] = False
+    assert bool((buf[keep] == 7.0).all())
+    # scores and gradient side by side in one buffer; in place in a padded one (its own alignment: sums in another order)
+    pair = torch.full((n, 2 * v + gap), 7.0, dtype=u.dtype, device="cuda")
+    pair[:, :v] = u
+    loss.value_and_gradient(pair[:, :v], out=pair[:, v + gap:])
+    assert torch.equal(pair[:, :v], u) and bool((pair[:, v:v + gap] == 7.0).all())
+    out2 = pair[:, v + gap:].clone()
+    loss.value_and_gradient(pair[:, :v], out=pair[:, :v])
+    assert torch.equal(pair[:, :v], out2) and torch.equal(pair[:, v + gap:], out2)
+    torch.testing.assert_close(out2, g, rtol=torch.finfo(u.dtype).eps, atol=2.0**-18)  # a rounding of each, and 64 * 2^-24 of terms up to 1 before
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_rows_far_apart(which):
+    """offsets that pass 32 bits, in elements and in bytes"""
+    (d, ud), (b, ub) = both_losses(n=4, v=300, e=60, dt=torch.bfloat16)
+    loss, u = ((d, ud), (b, ub))[which]
+    n, v = u.shape
+    ld = (1 << 30) + 24
+    buf = torch.empty(3 * ld + v, dtype=u.dtype, device="cuda")
+    far = buf.as_strided((n, v), (ld, 1))
+    far.copy_(u)
+    val, g = loss.value_and_gradient(u)
+    v2, g2 = loss.value_and_gradient(far, out=torch.empty_like(u))
+    torch.testing.assert_close(g2, g, rtol=2.0**-7, atol=1e-6)
+    assert v2 == pytest.approx(val, rel=1e-6)
+    loss.value_and_gradient(far, out=far)
+    assert torch.equal(far, g2)
+
+
+def test_another_current_stream():
+    for loss, u in both_losses():
+        val, g = loss.value_and_gradient(u)
+        s = torch.cuda.Stream()
+        for _ in range(4):
+            out, value = torch.full_like(u, 9.0), torch.zeros((), device="cuda")
+            late = torch.zeros_like(u)
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                big = torch.randn(2500, 2500, device="cuda")
+                for _ in range(8):
+                    big = big @ big * 1e-4
+                late.copy_(u + 0 * big[0, 0].nan_to_num(0.0, 0.0, 0.0))  # u is ready late, on s
+                value, out = loss.value_and_gradient_async(late, out=out, value=value)
+                got = out.clone()  # on s, behind the loss
+                v = value.clone()
+            s.synchronize()
+            assert torch.equal(got, g) and float(v) == pytest.approx(val, rel=2.0**-23)
+    made = torch.cuda.Stream()  # a loss made under one stream, used under another
+    with torch.cuda.stream(made):
+        (d, ud), (b, ub) = both_losses(seed=3)
+    torch.cuda.current_stream().wait_stream(made)
+    for (loss, u), (same, _) in zip(((d, ud), (b, ub)), both_losses(seed=3)):
+        assert torch.equal(loss.value_and_gradient(u)[1], same.value_and_gradient(u)[1])
+
+
+def test_recorded_and_replayed():
+    """each loss in two graphs, replayed in turn with eager calls of the same losses, and of others, between"""
+    m = pa()
+    ctx = m.Context.on_new_stream()
+    losses = both_losses(ctx=ctx)
+    big = both_losses(n=700, v=50, e=128, ctx=ctx, seed=1)  # the balance in tiles, with accumulators that take turns
+    wide = both_losses(n=2, v=40000, e=8, ctx=ctx, seed=2)  # the distillation in parts
+    torch.cuda.synchronize()
+    with torch.cuda.stream(ctx._stream_owner):
+        cases = []
+        for loss, u in (*losses, *big, *wide):
+            eager = loss.value_and_gradient(u)
+            second = loss.value_and_gradient(u * 0.5)
+            cases.append((loss, u.clone(), eager, second))
+        torch.cuda.synchronize()
+        graphs = []
+        for turn in range(2):
+            for loss, u, _, _ in cases:
+                out, value = torch.zeros_like(u), torch.zeros((), device="cuda")
+                torch.cuda.synchronize()
+                ctx.capture_begin()
+                loss.value_and_gradient_async(u, out=out, value=value)
+                graphs.append((ctx.capture_end(), out, value))
+        for k in range(4):
+            order = range(len(graphs)) if k % 2 else reversed(range(len(graphs)))
+            for i in order:
+                loss, u, eager, second = cases[i % len(cases)]
+                g, out, value = graphs[i]
+                g.launch()
+                torch.cuda.synchronize()
+                assert torch.equal(out, eager[1]) and float(value) == pytest.approx(eager[0], rel=2.0**-23)
+                out.fill_(3.0)
+                value.fill_(3.0)
+                if i % 3 == 0:
+                    v2, g2 = loss.value_and_gradient(u * 0.5)
+                    assert v2 == second[0] and torch.equal(g2, second[1])
+                if i % 5 == 0:
+                    float(u.sum())
+    with pytest.raises(m.ProxGradError):
+        ctx.capture_begin()
+        try:
+            losses[0][0].value_and_gradient_async(losses[0][1])  # needs an allocation
+        finally:
+            ctx.capture_end(abort=True)
+
+
+def test_somebody_elses_capture_is_refused():
+    m = pa()
+    for loss, u in both_losses():
+        want = loss.value_and_gradient(u)
+        out, value = torch.empty_like(u), torch.zeros((), device="cuda")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            w = u * 2
+            with pytest.raises(m.ProxGradError):
+                loss.value_and_gradient_async(u, out=out, value=value)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(w, u * 2)
+        v2, g2 = loss.value_and_gradient(u)
+        assert v2 == want[0] and torch.equal(g2, want[1])
+
+
+def test_refusals_on_the_device():
+    m = pa()
+    (d, ud), (b, ub) = both_losses()
+    for loss, u in ((d, ud), (b, ub)):
+        n, v = u.shape
+        buf = torch.zeros(4 * n * v, device="cuda")
+        part = lambda at, ld=v: buf[at:].as_strided((n, v), (ld, 1), at)  # noqa: E731
+        bad = [
+            (ValueError, (u[:-1], None)), (ValueError, (u[:, :-1], None)), (ValueError, (u.cpu(), None)), (TypeError, (u.int(), None)), (TypeError, (None, None)),
+            (TypeError, (u.cpu().numpy(), None)), (ValueError, (u, torch.empty(n + 1, v, device="cuda"))), (TypeError, (u, torch.empty_like(u, dtype=torch.float64))),
+            (ValueError, (u, torch.empty_like(u, device="cpu"))), (ValueError, (u.t().contiguous().t(), None)), (ValueError, (u[:1].expand(n, v), None)),
+            (ValueError, (part(0), part(4))), (ValueError, (part(4), part(0))), (ValueError, (part(0, v + 8), part(0))), (ValueError, (part(0), part(n * v - 1))),
+            (ValueError, (m.HIPVector.zeros(n * v + 1, np.float32), None)),
+            (TypeError, (u, m.HIPVector.zeros(n * v, np.float64))),
+            (ValueError, (m.HIPVector.zeros(n * v, np.float32, m.Context.on_new_stream()), None)),
+        ]
+        for err, (x, out) in bad:
+            with pytest.raises(err):
+                loss.value_and_gradient(x, out=out)
+        for value in (torch.zeros(2, device="cuda"), torch.zeros((), dtype=torch.float64, device="cuda"), torch.zeros(())):
+            with pytest.raises(ValueError):
+                loss.value_and_gradient_async(u, value=value)
+        val, g = loss.value_and_gradient(part(0), out=part(n * v))  # next to each other is fine
+        assert np.isfinite(val)
+    with pytest.raises(ValueError):
+        m.SlicedSeparableSum((d, b), ((0, ud.numel()), (0, ub.numel()))).value_and_gradient(m.HIPVector.zeros(ud.numel() + ub.numel(), np.float32))
+    half = m.HIPVector.zeros(64, np.float32)
+    with pytest.raises(ValueError):
+        m.SlicedSeparableSum((m.SqrNormL2(),), ((0, 32),)).value_and_gradient(half, out=half)  # the rest of x would be lost
+
+
+@pytest.mark.parametrize("n,e,k,groups", [(1, 1, 1, 1), (5000, 64, 6, 1), (3000, 256, 8, 1), (4000, 33, 2, 37), (2000, 1024, 16, 3)])
+def test_balance_many_tiles(n, e, k, groups):
+    """tiles in several accumulators, and the same bits each time"""
+    rng = np.random.default_rng(e)
+    x, xe = router(rng, n, e, torch.float32)
+    cut = np.sort(rng.integers(0, n + 1, groups - 1))
+    offsets = [0, *cut.tolist(), n]
+    loss = pa().BalanceLoss(n, e, k, offsets=offsets if groups > 1 else None, lam=2.0)
+    val, g = loss.value_and_gradient(x)
+    check_balance(loss, g, val, ref.balance(xe, k, offsets=offsets, lam=2.0), torch.float32)
+    for _ in range(5):
+        v2, g2 = loss.value_and_gradient(x)
+        assert v2 == val and torch.equal(g2, g)
+
+
+class OracleLoss:
+    is_generalized_quadratic = False
+
+    def __init__(self, parts):
+        self.parts = parts  # (lo, hi, rows -> (f, gradient))
+
+    def value_and_gradient(self, u):
+        f, g = 0.0, np.zeros_like(u)
+        for lo, hi, rows, fn in self.parts:
+            r = fn(u[lo:hi].reshape(rows, -1))
+            f += r[0]
+            g[lo:hi] = r[1].reshape(-1)
+        return f, g
+
+    def __call__(self, u):
+        return self.value_and_gradient(u)[0]
+
+
+def routed_student(rng, tokens=12, v=30, e=8, k=2, top=5, dim=25):
+    """scores and router logits of one linear model: A x holds the distillation's rows, then a gap, then the router's"""
+    t, idx = teacher(rng, tokens, v, top)
+    y = rng.integers(0, v, tokens)
+    lse = np.log(np.exp(t / 2).sum(1) + 0.5)
+    a, b = tokens * v, tokens * v + 8
+    kw = dict(temperature=2.0, lam=4.0, teacher_lse=lse, labels=y, label_lam=0.5)
+    A = rng.normal(size=(b + tokens * e + 4, dim)) / np.sqrt(dim)
+    dist = pa().DistillationLoss(t, idx, v, **{**kw, "teacher_lse": lse.astype(np.float64)})
+    bal = pa().BalanceLoss(tokens, e, k, offsets=[0, 5, tokens], lam=0.1)
+    f = pa().SlicedSeparableSum((dist, bal), ((0, a), (b, b + tokens * e)))
+    fo = OracleLoss([(0, a, tokens, lambda r: ref.distillation(r, t, idx, **kw)[:2]),
+                     (b, b + tokens * e, tokens, lambda r: ref.balance(r, k, offsets=[0, 5, tokens], lam=0.1)[:2])])
+    return f, fo, A
+
+
+def test_the_sum_of_both_on_one_vector():
+    m = pa()
+    f, fo, A = routed_student(np.random.default_rng(0))
+    u = np.random.default_rng(1).normal(size=A.shape[0])
+    want = fo.value_and_gradient(u)
+    ud = m.HIPVector.from_numpy(u)
+    val, g = f.value_and_gradient(ud)
+    assert isinstance(val, np.float64) and val == pytest.approx(want[0], rel=1e-12) and f(ud) == val
+    np.testing.assert_allclose(g.numpy(), want[1], rtol=1e-11, atol=1e-13)  # some hundred roundings of 2^-53 of terms up to 4
+    assert not f.is_convex and not f.is_generalized_quadratic
+    # against differences: second order in h, the third derivatives along d are below 30
+    d = np.random.default_rng(2).normal(size=u.size)
+    d /= np.linalg.norm(d)
+    h = 1e-5
+    diff = (f(m.HIPVector.from_numpy(u + h * d)) - f(m.HIPVector.from_numpy(u - h * d))) / (2 * h)
+    assert abs(diff - float(want[1] @ d)) <= 30 * h * h / 6 + 2.0**-52 * 64 * abs(want[0]) / h
+
+
+@pytest.mark.parametrize("name", ["ForwardBackwardIteration", "FastForwardBackwardIteration", "PANOCIteration"])
+def test_iterations_on_both_together(name):
+    """one objective of both losses behind a linear model, next to the same iteration in numpy on the oracle's losses"""
+    m = pa()
+    f, fo, A = routed_student(np.random.default_rng(4))
+    x0 = np.zeros(A.shape[1])
+    kw = dict(x0=x0, gamma=0.05)
+    if name == "PANOCIteration":
+        it = m.PANOCIteration(f=f, A=A, g=m.NormL1(0.01), adaptive=True, **kw)
+        ora = o.PANOCIteration(f=fo, A=A, g=o.NormL1(0.01), adaptive=True, **kw)
+    else:
+        it = getattr(m, name)(f=m.Composed(f, A), g=m.NormL1(0.01), **kw)
+        ora = getattr(o, name)(f=o.Composed(fo, A), g=o.NormL1(0.01), **kw)
+    for a, b in itertools.islice(zip(it, ora), 12):
+        assert float(a.gamma) == pytest.approx(float(b.gamma), rel=1e-12)
+        np.testing.assert_allclose(a.z.numpy(), b.z, rtol=1e-8, atol=1e-9)
