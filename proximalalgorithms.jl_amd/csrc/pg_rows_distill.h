@@ -106,14 +106,14 @@ __device__ __forceinline__ void entry_p(const DArgs& a, int64_t row, int k, doub
   p = ex2(lp * (C)LOG2E);
 }
 
-// ---- a row's place in memory: head elements up to the first 16-byte boundary, whole vectors, tail -----------------
-template <typename T>
+// ---- a row's place in memory: head elements up to the first boundary of ALIGN bytes, whole 16-byte vectors, tail -----------------
+template <typename T, int ALIGN = 16>
 struct Place {
   int h, nmain, hV;
   __device__ __forceinline__ Place(const T* xr, int V) {
     constexpr int N = Elem<T>::N;
-    const int off = (int)((reinterpret_cast<uintptr_t>(xr) & 15u) / sizeof(T));
-    h = off ? N - off : 0;
+    const int off = (int)((reinterpret_cast<uintptr_t>(xr) & (ALIGN - 1u)) / sizeof(T));
+    h = off ? ALIGN / (int)sizeof(T) - off : 0;
     h = h < V ? h : V;
     nmain = (V - h) / N;
     hV = h + nmain * N;
@@ -141,11 +141,21 @@ __device__ __forceinline__ void power(int squares, const C (&x)[N], const C (&e)
     for (int i = 0; i < N; ++i) what(i, ex2((x[i] - m) * (C)LOG2E));
   }
 }
-// e, or 0 if bit i is set
-__device__ __forceinline__ float without(float e, unsigned bits, int i) {
-  return __builtin_bit_cast(float, __builtin_bit_cast(int, e) & ~((int)(bits << (31 - i)) >> 31));
+// e[i] = 0 where bit i is clear (two operations each; written in C they become a test, a comparison and a choice)
+template <int I = 0, int N>
+__device__ __forceinline__ void keep(float (&e)[N], unsigned bits) {
+  if constexpr (I < N) {
+    int m;
+    asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(m) : "v"(bits), "n"(I));
+    e[I] = __builtin_bit_cast(float, __builtin_bit_cast(int, e[I]) & m);
+    keep<I + 1>(e, bits);
+  }
 }
-__device__ __forceinline__ double without(double e, unsigned bits, int i) { return (bits >> i) & 1u ? 0.0 : e; }
+template <int N>
+__device__ __forceinline__ void keep(double (&e)[N], unsigned bits) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = (bits >> i) & 1u ? e[i] : 0.0;
+}
 
 // Sums of one thread, relative to a reference score m that is one of the row's (or the type's lowest value while there is
 // none): any score will do that is not far below the largest, so m is raised rarely, by a branch.  Far:
@@ -186,10 +196,7 @@ struct Run {
       s1 += t[0] + t[1];
     }
     if constexpr (TAIL) {
-      if (bits) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) e[i] = without(e[i], bits, i);
-      }
+      if (bits) keep(e, ~bits);
     }
 #pragma unroll
     for (int o = 1; o < N; o *= 2)
@@ -497,6 +504,8 @@ pg_status run_parts(pg_ctx* c, DArgs a, int64_t rows) {
 // registers and, as a vector leaves, loads the same vector of the group's NEXT row in its place, so that the memory pipes
 // stay busy through the reduction.  Loads return in order, so nothing may be asked for between those loads and pass 1 that
 // is needed before it: the next row's list is asked for a pass ahead and waits in LDS, and no register may spill there.
+// A workgroup's vectors start at a 128-byte line of the scores, and of the gradient where its rows lie alike, or each wave's
+// access ends in two half lines (2048 x 131000 bf16: both on a line 235 us, one of them 246, both 8 bytes off 257).
 template <typename T, int NT, int NV>
 struct RowsGeom {
   using C = typename Elem<T>::C;
@@ -504,7 +513,9 @@ struct RowsGeom {
   static constexpr int WG = NT < 256 ? 256 : NT;
   static constexpr int GPW = WG / NT, NW = NT / 64;
   static constexpr int capacity = NT * NV * N;  // classes a group's registers hold
-  static __host__ __device__ int words(int V) { return ((V + BIT0 + N + 31) / 32 + 1) & ~1; }
+  static constexpr int ALIGN = NT == 64 ? 16 : 128;
+  static constexpr int FRONT = NT == 64 ? BIT0 : 64;  // bits in front of the first vector's: at least its head
+  static __host__ __device__ int words(int V) { return ((V + FRONT + N + 31) / 32 + 1) & ~1; }
   // two bitmaps and two lists (this row's, the next's) of scores and classes, one of logits and of probabilities
   static __host__ __device__ int group_bytes(int V, int K) { return words(V) * 8 + (K * (4 * (int)sizeof(C) + 8) + 7) / 8 * 8; }
 };
@@ -516,6 +527,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
   const PG_CONST_AS DArgs* ap = (const PG_CONST_AS DArgs*)__builtin_amdgcn_kernarg_segment_ptr();
 #define a (*ap)
   using G = RowsGeom<T, NT, NV>;
+  using P = Place<T, G::ALIGN>;
   using C = typename G::C;
   constexpr int N = G::N, NW = G::NW, GPW = G::GPW;
   constexpr int AGAIN = 1 << 30;  // marks a list entry whose class an earlier one holds
@@ -546,7 +558,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     for (; row < a.nrows; row += stride) {
       if (a.w == nullptr || (w = ld_real_u(a.w, a.wdt, row)) != 0.0) break;
       T* gr = (T*)a.g + row * a.ldg;
-      const Place<T> pl(gr, a.V);
+      const P pl(gr, a.V);
       const u32x4 zero = {0u, 0u, 0u, 0u};
 #pragma clang loop unroll(disable)
       for (int v = tid; v < pl.nmain; v += NT) st16(at16(gr + pl.h, v), zero);
@@ -581,12 +593,12 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
   auto put_list = [&](int64_t row, int id, RawReal<C> t, int y, T x, T xy, int par, int slot) {
     if (row >= a.nrows) return;
     const T* xr = (const T*)a.x + row * a.ldx;
-    const Place<T> pl(xr, a.V);
+    const P pl(xr, a.V);
     unsigned* bm = bm0 + par * nwords;
     auto put = [&](int k, int id, C t, T x) {
       int mark = 0;
       if (id >= 0) {
-        const int b = id - pl.h + BIT0;
+        const int b = id - pl.h + G::FRONT;
         const unsigned bit = 1u << (b & 31);
         if (atomicOr(&bm[b >> 5], bit) & bit) {
           mark = AGAIN;
@@ -607,7 +619,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     if (tid == NT - 1) sxy[grp][par] = up<T>(xy);
   };
   // head elements: threads 0 ..; tail elements: threads NT - 1 .. down
-  auto edge_of = [&](const Place<T>& pl) { return tid < pl.h ? tid : (pl.hV + (NT - 1 - tid) < a.V ? pl.hV + (NT - 1 - tid) : -1); };
+  auto edge_of = [&](const P& pl) { return tid < pl.h ? tid : (pl.hV + (NT - 1 - tid) < a.V ? pl.hV + (NT - 1 - tid) : -1); };
 
   u32x4 d[NV];
   T edge = (T)0.f;
@@ -625,7 +637,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     ask_scores(row, id, y, x, xy);
     if (row < a.nrows) {
       const T* xr = (const T*)a.x + row * a.ldx;
-      const Place<T> pl(xr, a.V);
+      const P pl(xr, a.V);
       const int ee = edge_of(pl);
       if (ee >= 0) edge = xr[ee];
       const __amdgpu_buffer_rsrc_t rx = row_rsrc(xr + pl.h, pl.nmain * 16);
@@ -641,9 +653,9 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     asm volatile("" : "+s"(ap));
     const T* xr = (const T*)a.x + row * a.ldx;
     T* gr = (T*)a.g + row * a.ldg;
-    const Place<T> pl(xr, a.V);
+    const P pl(xr, a.V);
     const int ee = edge_of(pl);
-    const int bbase = pl.h - BIT0;
+    const int bbase = pl.h - G::FRONT;
     unsigned* bm = bm0 + par * nwords;
     const C* lx = lx0 + par * K;
     const int* li = li0 + par * K;
@@ -689,7 +701,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
         }
         C f[N];
         unpack<T>(d[j], f);
-        run.template add<N>(f, tail ? listed_bits<T>(bm, min(j * NT + t0, pl.nmain) * N + BIT0) : 0u);
+        run.template add<N>(f, tail ? listed_bits<T>(bm, min(j * NT + t0, pl.nmain) * N + G::FRONT) : 0u);
       }
     }
     if (ee >= 0) {
@@ -756,7 +768,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     asm volatile("" : "+s"(ap));
     const bool more = nrow < a.nrows;
     const T* xn = (const T*)a.x + (more ? nrow : row) * a.ldx;
-    const Place<T> pn(xn, a.V);
+    const P pn(xn, a.V);
     const int en = edge_of(pn), next_main = more ? pn.nmain : 0;
     const __amdgpu_buffer_rsrc_t rg = row_rsrc(gr + pl.h, pl.nmain * 16), rn = row_rsrc(xn + pn.h, next_main * 16);
     T edge_next = (T)0.f;
