@@ -8,7 +8,7 @@
 // R3L row groups per wave (LDS again: 8 R3L KiB), and the twelve fp64 scalar accumulators, which only the writer lanes of wave 0
 // touch, in LDS as well (in registers they cost every lane 24 and the kernel spilled); the three image accumulator sets and
 // the tile in registers.  Per column and instance the arithmetic is gemv_tnm_pair_kernel's except that a lane's part of a dot runs as
-// two partial sums (even / odd elements, v_pk_fma_f32 in Float32): results equal the single sweep's to rounding, like the pair's.
+// two partial sums (even / odd elements): results equal the single sweep's to rounding, like the pair's.
 #include <mutex>
 
 #include "pg_gemv_tn.h"
@@ -100,8 +100,8 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_tnm_trio_kernel(TNArgs<T> a, 
   auto process = [&](const Tile& t, int64_t cg, int buf) __attribute__((always_inline)) {
     const int64_t j0 = cg * C;
     T dot[3][C];
-    // two partial sums per instance, column and lane (even / odd elements): Float32 runs them as v_pk_fma_f32, half the issue
-    // slots of the single sweep's one chain -- with three instances on a tile the dots are what the step waits for.  Row groups
+    // two partial sums per instance, column and lane (even / odd elements): two chains instead of the single sweep's one -- with
+    // three instances on a tile the dots are what the step waits for.  Row groups
     // outermost: a slice entry is read from LDS once for the C columns of the step.
     T2 dd[3][C];
 #pragma unroll

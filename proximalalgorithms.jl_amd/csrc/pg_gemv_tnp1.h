@@ -9,7 +9,7 @@
 // in every lane, one column after the other, with its branches; the member-order sum was a v_readlane + v_add per member and
 // column behind a jump table; the column map was evaluated three times; the wave sum crossed LDS twice per column and the
 // partial dots once more (five exposed LDS round trips per step).  Here:
-//   * dots as packed partial sums (v_pk_fma_f32: two multiply-adds per instruction), reduced ACROSS the C columns at once
+//   * dots as two partial sums each (even / odd elements), reduced ACROSS the C columns at once
 //     (cr_stage, pg_lanes.h: permlane swaps and DPP moves, no LDS);
 //   * the step's granules are summed over the members by DPP row shifts -- lane c*G of every 16-lane row adds the lanes
 //     c*G + k*C*G of its row, k ascending (= member order), rows combined by two permlane swaps -- TM - 1 adds for all columns

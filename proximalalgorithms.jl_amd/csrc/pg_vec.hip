@@ -386,8 +386,7 @@ struct DRBlockArgs {
   double gscale;
 };
 
-// two elements side by side: on gfx950 the multiply-adds of a Float32 pair issue as ONE v_pk_fma_f32 / v_pk_mul_f32 /
-// v_pk_add_f32 (Float64 pairs are two instructions; same source)
+// two elements side by side, in lockstep: two dependency chains
 template <typename T>
 struct Pair2 {
   typedef T type __attribute__((ext_vector_type(2)));
@@ -443,8 +442,7 @@ __device__ __forceinline__ void dr_block_compute(const DRBlockArgs<T, GKIND, K>&
     const P two = {T(2), T(2)}, gam = {a.gamma, a.gamma};
     // sepquad_prepare / sepquad_apply on pairs: same operations, same rounding, per lane.  The NP pairs of a vector advance
     // in lockstep (pair loop INSIDE the iteration loop): consecutive instructions then belong to different dependency
-    // chains, which is what the packed-Float32 pipeline wants (a dependent v_pk_* needs a wait state; written pair by
-    // pair the compiler filled those with s_nop, 276 of them against 358 arithmetic instructions).
+    // chains.
     // Float32 quotient a / den = RN32(RN64(a * RN64(1 / den))): the double product is within 2^-52 of a / den, and the
     // quotient of two 24-bit significands is never closer than 2^-49 (relative) to a rounding boundary of the 24-bit
     // format, so the final rounding lands on RN32(a / den) -- the bits of the IEEE division, for three full-rate
@@ -476,8 +474,7 @@ __device__ __forceinline__ void dr_block_compute(const DRBlockArgs<T, GKIND, K>&
         for (int p = 0; p < NP; ++p) qq[p] = (P){(T)((double)aa[p][0] * inv64[p][0]), (T)((double)aa[p][1] * inv64[p][1])};
       } else {
         // The scheduling fences keep the pairs in lockstep in the EMITTED code too: in the prefetching loop the scheduler
-        // otherwise runs one pair's whole chain after the other's and pads every dependent v_pk_* with s_nop (four per
-        // iteration, ~8 % of the loop's issue cycles)
+        // otherwise runs one pair's whole chain after the other's
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int p = 0; p < NP; ++p) qq[p] = aa[p] * inv[p];
