@@ -293,9 +293,9 @@ class DistillationLoss(_RowLoss):
 def _balance_tiles(tokens, experts, offsets, num_cu):
     """(rows of (begin, end, group, part), tokens of a tile, whether each group is one tile): an evaluation in pieces of one group each.
 
-    Small groups take a workgroup each and one launch; 64 tokens of 64 experts take 7 us that way and 9 in tiles, 64 of 256 experts 15
-    and 13.5.  Else a tile is four waves' work, at least a step of theirs: four tiles per compute unit (131072 x 256: 107 us; two 117,
-    eight 110), no fewer than 16 tokens in one (256 x 256: 14 us; 32 tokens 18, 64 tokens 25)."""
+    Small groups take a workgroup each and one launch; 64 tokens of 64 experts take 7.4 us that way and 9.9 in tiles, 64 of 256 experts 14.0
+    and 14.2.  Else a tile is four waves' work, at least a step of theirs: four tiles per compute unit (131072 x 256: 94 us; two 103,
+    eight 95), no fewer than 16 tokens in one (256 x 256: 14.4 us; 32 tokens 18.7, 64 tokens 27.4)."""
     offsets = np.asarray(offsets, np.int64)
     lengths = np.diff(offsets)
     longest = int(lengths.max(initial=0))
