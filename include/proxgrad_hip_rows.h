@@ -43,8 +43,8 @@ enum { PG_BF16 = 2, PG_F16 = 3 }; /* beside PG_F32, PG_F64: understood by this h
  *   L = sum_k p_k (log p_k - log q_{i_k}) + p_r (log p_r - log sum_{v not in S} q_v)
  *   f = lam sum_n w_n L_n + label_lam sum_n w_n (log sum_v exp x_{n,v} - x_{n,y_n})     (y = -1: no label; labels may be NULL)
  * A class listed twice counts with both entries.  0 log 0 = 0.  A row of w = 0 is not read, its gradient is zero.  A row whose
- * scores are all -inf contributes nothing.  A listed class or a label at score -inf makes f = +inf where its mass is not zero,
- * and leaves the gradient finite.  A NaN among a row's scores, or an index or label outside [-1, classes), makes f and that
+ * scores are all -inf contributes nothing.  A listed class, a label or all that is outside the list at score -inf makes f = +inf
+ * where its mass and its factor (lam, label_lam) are not zero, and leaves the gradient finite.  A NaN among a row's scores, or an index or label outside [-1, classes), makes f and that
  * row's gradient NaN. */
 typedef struct pg_distill {
   int64_t rows, classes, top; /* classes <= 2^24, top <= 1024 */

@@ -69,11 +69,11 @@ def distillation(x, t, idx, *, temperature=1.0, lam=1.0, teacher_lse=None, weigh
             row = terms.sum() + (pr * (np.log(pr) - np.log(qr)) if pr > 0 else 0.0)
             row_size = sizes[np.isfinite(sizes)].sum() + (64 * pr * (1 + abs(np.log(pr)) + abs(np.log(qr))) + 64 * (1 + abs(np.log(qr))) if pr > 0 and qr > 0 else 0.0)
             row_size += left_size * (1 + abs(np.log(pr)) + abs(np.log(qr))) if pr > 0 and qr > 0 and left_size else 0.0
-        f += lam * w * row
+        f += lam * w * row if lam else 0  # (a term that is switched off adds nothing, an infinite one neither)
         f_size += lam * w * row_size
         grad[i] = lam * w / temperature * (mass * q - phat - rest * q)
         size[i] = lam * w / temperature * ((mass + rest) * q * (64 + 6 * far / temperature) + ksize)
-        if y >= 0:
+        if y >= 0 and label_lam:
             ls = _log_softmax(x[i])
             one = np.zeros(v, L)
             one[y] = 1

@@ -432,7 +432,7 @@ __global__ __launch_bounds__(PT) void distill_part_grad(DArgs a) {
       C lp, p;
       entry_p<C>(a, q.row, k, norm, lp, p);
       const C x = (C)xk[k];
-      if (q.part == 0 && !rs.empty && p != C(0)) v_row += a.lam * w * (double)(p * (lp - ((x - rs.M) * (C)a.invT - rs.ls)));
+      if (q.part == 0 && !rs.empty && p != C(0) && a.lam != 0.0) v_row += a.lam * w * (double)(p * (lp - ((x - rs.M) * (C)a.invT - rs.ls)));
       if (q.has(id)) {
         C ph = p;
         bool owner = true;
@@ -454,8 +454,8 @@ __global__ __launch_bounds__(PT) void distill_part_grad(DArgs a) {
         if (!((bm[b >> 5] >> (b & 31)) & 1u)) gr[y] = (T)(entry((C)xk[a.K], rs.cR) - rs.qy);
       }
       if (q.part == 0 && !rs.empty) {
-        if (TAIL && rs.pr != 0.0) v_row += a.lam * w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - rs.log_qr);
-        if (y >= 0 && y < a.V) v_row += a.lab_lam * w * (double)(rs.ls1 - ((C)xk[a.K] - rs.M));
+        if (TAIL && rs.pr != 0.0 && a.lam != 0.0) v_row += a.lam * w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - rs.log_qr);
+        if (y >= 0 && y < a.V && a.lab_lam != 0.0) v_row += a.lab_lam * w * (double)(rs.ls1 - ((C)xk[a.K] - rs.M));
       }
       if (rs.ls != rs.ls) v_row = NAN;  // a NaN score, or an index or label out of range
     }
@@ -824,7 +824,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
         const double t = (double)lt[k] * a.invT;
         const C l = t == -INFINITY ? (C)t : (C)(t - norm);  // (a list of -inf only has no norm)
         p = ex2(l * (C)LOG2E);
-        if (p != C(0) && !rs.empty) v_acc += a.lam * w * (double)(p * (l - ((lx[k] - rs.M) * (C)a.invT - rs.ls)));
+        if (p != C(0) && !rs.empty && a.lam != 0.0) v_acc += a.lam * w * (double)(p * (l - ((lx[k] - rs.M) * (C)a.invT - rs.ls)));
         bm[((id & ~AGAIN) - bbase) >> 5] = 0;
       }
       lp[k] = p;
@@ -848,9 +848,9 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
       if (y >= 0) {
         const C xy = sxy[grp][par];
         if (!flags[grp][slot][1]) gr[y] = (T)(entry(xy, rs.cR) - rs.qy);
-        if (!rs.empty) v_acc += a.lab_lam * w * (double)(rs.ls1 - (xy - rs.M));
+        if (!rs.empty && a.lab_lam != 0.0) v_acc += a.lab_lam * w * (double)(rs.ls1 - (xy - rs.M));
       }
-      if (tail && rs.pr != 0.0 && !rs.empty) v_acc += a.lam * w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - rs.log_qr);
+      if (tail && rs.pr != 0.0 && !rs.empty && a.lam != 0.0) v_acc += a.lam * w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - rs.log_qr);
       if (rs.ls != rs.ls) v_acc = NAN;  // a NaN score, or an index or label out of range
     }
     edge = edge_next;

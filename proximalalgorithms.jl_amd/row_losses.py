@@ -8,7 +8,7 @@ tensor on the device (Float32, Float64, bfloat16 or Float16; rows any distance a
 
 A loss runs on its context's stream.  Called under another current torch stream, it waits for that stream's work and that
 stream waits for the loss.  One host thread per context at a time; a graph is recorded with ``Context.capture_begin`` (with ``out``
-and ``value`` given: nothing can be allocated while recording)."""
+and ``value`` given: nothing can be allocated while recording) and works on the loss's own buffers: keep the loss as long as the graph."""
 import ctypes as C
 
 import numpy as np

@@ -285,6 +285,33 @@ def test_somebody_elses_capture_is_refused():
         assert v2 == want[0] and torch.equal(g2, want[1])
 
 
+def test_a_capture_of_the_contexts_own_stream_by_somebody_else_is_refused():
+    m = pa()
+    ctx = m.Context.on_new_stream()
+    for loss, u in both_losses(ctx=ctx):
+        out, value = torch.empty_like(u), torch.zeros((), device="cuda")
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=ctx._stream_owner):
+            w = u * 3
+            with pytest.raises(m.ProxGradError):
+                loss.value_and_gradient_async(u, out=out, value=value)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(w, u * 3)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(ctx._stream_owner):
+            assert np.isfinite(loss.value_and_gradient(u)[0])
+    ctx.capture_begin()
+    try:
+        with pytest.raises(m.ProxGradError):
+            m.BalanceLoss(4, 4, 2, ctx=ctx)
+        with pytest.raises(m.ProxGradError):
+            m.DistillationLoss(np.zeros((2, 1)), np.zeros((2, 1), int), 4, ctx=ctx)
+    finally:
+        ctx.capture_end(abort=True)
+
+
 def test_refusals_on_the_device():
     m = pa()
     (d, ud), (b, ub) = both_losses()
@@ -329,6 +356,62 @@ def test_balance_many_tiles(n, e, k, groups):
     for _ in range(5):
         v2, g2 = loss.value_and_gradient(x)
         assert v2 == val and torch.equal(g2, g)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n,v", [(6, 300), (1, 70000)])
+def test_masked_classes_and_terms_that_are_switched_off(dtype, n, v):
+    """the list, the label or everything outside the list at -inf: an infinite value, unless that term's factor is zero; finite gradients"""
+    rng = np.random.default_rng(3)
+    t, idx = teacher(rng, n, v, 5)
+    td, te = tdev(t, torch.float32)
+    x, xe = scores(rng, n, v, DT[dtype], idx, t)
+    y = idx[:, 1].copy()
+    rows = np.arange(n)
+    lse = np.log(np.exp(te).sum(1) + 3.0).astype(np.float32)
+    for where in ("list", "outside"):
+        xm = x.clone()
+        if where == "list":
+            xm[torch.from_numpy(rows).cuda(), torch.from_numpy(idx[:, 1]).cuda()] = float("-inf")  # a listed class, and the label
+        else:
+            keep = torch.zeros(n, v, dtype=torch.bool, device="cuda").scatter_(1, torch.from_numpy(idx).cuda(), True)
+            xm[~keep] = float("-inf")
+        xe = xm.double().cpu().numpy()
+        for lam, label_lam, rest in itertools.product((0.0, 1.5), (0.0, 0.5), (False, True)):
+            kw = dict(lam=lam, label_lam=label_lam)
+            f = pa().DistillationLoss(td, torch.from_numpy(idx).cuda(), v, labels=torch.from_numpy(y).cuda(), teacher_lse=torch.from_numpy(lse).cuda() if rest else None, **kw)
+            val, g = f.value_and_gradient(xm)
+            want = ref.distillation(xe, te, idx, labels=y, teacher_lse=lse.astype(np.float64) if rest else None, **kw)
+            assert np.isinf(want[0]) == bool((where == "list" and (lam or label_lam)) or (where == "outside" and rest and lam))
+            check(g, val, want, DT[dtype])
+
+
+def test_balance_of_nothing_and_positions_on_the_device():
+    m = pa()
+    for offsets in (None, [0], [0, 0, 0]):
+        loss = m.BalanceLoss(0, 4, 2, offsets=offsets)
+        val, g = loss.value_and_gradient(torch.empty(0, 4, device="cuda"))
+        assert val == 0.0 and g.shape == (0, 4) and not loss.counts.any()
+    rng = np.random.default_rng(0)
+    x, xe = router(rng, 50, 12, torch.float32)
+    offsets = torch.tensor([0, 7, 7, 50], device="cuda", dtype=torch.int32)
+    mask = torch.from_numpy((rng.random(50) < 0.5).astype(np.uint8) * 255).cuda()
+    loss = m.BalanceLoss(50, 12, 3, offsets=offsets, mask=mask)
+    val, g = loss.value_and_gradient(x)
+    check_balance(loss, g, val, ref.balance(xe, 3, offsets=[0, 7, 7, 50], mask=mask.cpu().numpy() > 0), torch.float32)
+    mask.fill_(1)  # tensors on the device are used where they are
+    val, g = loss.value_and_gradient(x)
+    check_balance(loss, g, val, ref.balance(xe, 3, offsets=[0, 7, 7, 50]), torch.float32)
+    empty = loss(x)
+    assert empty == val
+    mask.fill_(0)
+    val, g = loss.value_and_gradient(x)
+    assert val == 0.0 and not g.any() and not loss.counts.any()
+    for dt in DT.values():  # one loss, scores of any type
+        mask.fill_(1)
+        xd = x.to(dt)
+        val, g = loss.value_and_gradient(xd)
+        check_balance(loss, g, val, ref.balance(xd.double().cpu().numpy(), 3, offsets=[0, 7, 7, 50]), dt)
 
 
 class OracleLoss:
