@@ -9,7 +9,7 @@
  *
  * Element types: scores and gradients are PG_F32, PG_F64, PG_BF16 or PG_F16.  Arithmetic, softmax statistics and sums are
  * Float32 for the three narrow types and Float64 for PG_F64; the total over the rows is Float64; each gradient entry is
- * rounded to the scores' type once.  In Float32 a probability of less than 2^-126 of the row's largest is 0.
+ * rounded to the scores' type once.  In Float32 a probability of less than 2^-97 of the row's largest may be 0.
  *
  * Rows are `ld` elements apart (ld >= the row's length), elements of a row are adjacent, no alignment is asked for beyond
  * the element's own.  What lies between the rows is neither read nor written.  grad may be the scores' own buffer (same

@@ -48,31 +48,34 @@ def distillation(x, t, idx, *, temperature=1.0, lam=1.0, teacher_lse=None, weigh
         np.add.at(phat, cls, p)
         with np.errstate(invalid="ignore"):
             np.add.at(ksize, cls, np.where(p > 0, p * (64 + 4 * np.abs(lp)), 0.0))
-        pr, rest, left_size = L(0), np.zeros(v, L), L(0)
+        pr, log_qr, left_size, share, near = L(0), L(0), L(0), np.zeros(v, L), np.zeros(v, L)
         outside = np.ones(v, bool)
         outside[cls] = False
         if teacher_lse is not None and len(tt) and outside.any():
             pr = max(L(0), L(1) - p.sum())
-            qr = q[outside].sum()
-            rest[outside] = pr / qr if qr > 0 else 0.0
+            top = lq[outside].max()
+            log_qr = top + np.log(np.exp(lq[outside] - top).sum()) if top > -np.inf else -L(np.inf)
+            if top > -np.inf:  # the outside class's mass is divided by the softmax of its own classes, however little q leaves them
+                share[outside] = np.exp(lq[outside] - top) / np.exp(lq[outside] - top).sum()
+                near[outside] = np.where(share[outside] > 0, (top - lq[outside]) * temperature * log2e, 0.0)
             # 1 - sum p is as far off as the sum is, (64 + 4 |log p|) roundings of each p, however little is left; an entry outside
             # the list gets q / Q of that, the value its slope log pr - log Q + 1 times that
             left_size = (p[p > 0] * (64 + 4 * np.abs(lp[p > 0]))).sum()
-            if qr > 0:
-                ksize[outside] += left_size * q[outside] / qr
+            ksize[outside] += left_size * share[outside]
         elif teacher_lse is not None and len(tt) == 0:
-            pr, qr, rest = L(1), L(1), np.ones(v, L)  # nothing listed: the outside class is everything on both sides
+            pr, log_qr, share = L(1), L(0), q  # nothing listed: the outside class is everything on both sides
+            near = far
         mass = p.sum() + pr
         with np.errstate(invalid="ignore", divide="ignore"):
             terms = np.where(p > 0, p * (lp - lq[cls]), 0.0)
             sizes = np.where(p > 0, p * (64 + 8 * (np.abs(lp) + np.abs(lq[cls]) + np.abs(x[i][cls]) / temperature)), 0.0)
-            row = terms.sum() + (pr * (np.log(pr) - np.log(qr)) if pr > 0 else 0.0)
-            row_size = sizes[np.isfinite(sizes)].sum() + (64 * pr * (1 + abs(np.log(pr)) + abs(np.log(qr))) + 64 * (1 + abs(np.log(qr))) if pr > 0 and qr > 0 else 0.0)
-            row_size += left_size * (1 + abs(np.log(pr)) + abs(np.log(qr))) if pr > 0 and qr > 0 and left_size else 0.0
+            row = terms.sum() + (pr * (np.log(pr) - log_qr) if pr > 0 else 0.0)
+            row_size = sizes[np.isfinite(sizes)].sum() + (64 * pr * (1 + abs(np.log(pr)) + abs(log_qr)) + 64 * (1 + abs(log_qr)) if pr > 0 and log_qr > -np.inf else 0.0)
+            row_size += left_size * (1 + abs(np.log(pr)) + abs(log_qr)) if pr > 0 and log_qr > -np.inf else 0.0
         f += lam * w * row if lam else 0  # (a term that is switched off adds nothing, an infinite one neither)
         f_size += lam * w * row_size
-        grad[i] = lam * w / temperature * (mass * q - phat - rest * q)
-        size[i] = lam * w / temperature * ((mass + rest) * q * (64 + 6 * far / temperature) + ksize)
+        grad[i] = lam * w / temperature * (mass * q - phat - pr * share)
+        size[i] = lam * w / temperature * (mass * q * (64 + 6 * far / temperature) + pr * share * (64 + 6 * near / temperature) + ksize)
         if y >= 0 and label_lam:
             ls = _log_softmax(x[i])
             one = np.zeros(v, L)

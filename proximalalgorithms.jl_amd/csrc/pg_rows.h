@@ -188,7 +188,7 @@ __device__ __forceinline__ int64_t ld_int_u(const void* p, int bits, int64_t i) 
 __device__ __forceinline__ float uniform(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))); }
 __device__ __forceinline__ double uniform(double v) { return pg_readlane(v, 0); }
 
-// (one instruction; results below 2^-126 are 0)
+// (one instruction; results below 2^-126 are 0: an exponent of 20 below the largest's, 2^-97 of it)
 __device__ __forceinline__ float ex2(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ double ex2(double v) { return exp2(v); }
 __device__ __forceinline__ float lg2(float v) { return __builtin_amdgcn_logf(v); }

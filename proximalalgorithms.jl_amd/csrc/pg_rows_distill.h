@@ -27,7 +27,7 @@ pg_status distill_f16(pg_ctx* c, const DArgs& a, int64_t rows);
 constexpr double LOG2E = 1.4426950408889634;
 constexpr double LN2 = 0.6931471805599453;
 constexpr int BIT0 = 8;         // bits in front of a chunk's first aligned vector (the head of a misaligned row: at most 7)
-constexpr int STAT = 6;         // doubles per (row, part)
+constexpr int STAT = 8;         // doubles per (row, part)
 constexpr int MAX_PARTS = 64;   // one lane each when a row's parts are joined
 constexpr int MAX_TOP = 1024;
 constexpr int PART_BITS = 32 * 1024 * 8;                          // classes of a part: its bitmap takes 32 KiB of LDS
@@ -53,52 +53,84 @@ namespace {
 
 // ---- one row's scalars, from the statistics over the whole row ----------------------------------------------------
 template <typename C>
+struct Sums {  // of exp((x - m) / T) and exp(x - m)
+  C m, s, s1;
+  static __device__ __forceinline__ Sums none() { return {Lim<C>::lowest, C(0), C(0)}; }
+};
+template <typename C>
 struct RowScal {
-  C M, cB, cR, c1;  // reference score; coefficients of e at listed / unlisted classes, of exp(x - M) for labels at T != 1
-  C ql, qy;         // what a unit of teacher mass / the label takes off
-  C ls, ls1;        // log sum exp((x - M) / T) and log sum exp(x - M)
-  double pr, log_qr;
+  C M, Mu;           // reference scores: of the row, of the unlisted classes (the same where the list is no class of its own)
+  C cB, cR, c1, c1u; // coefficients: of exp((x - M) / T) at listed classes, of exp((x - Mu) / T) at the others, of exp(x - M), exp(x - Mu) for labels at T != 1
+  C ql, qy;          // what a unit of teacher mass / the label takes off
+  C S, S1, Su;       // sums of exp((x - M) / T), exp(x - M), and over the unlisted of exp((x - Mu) / T)
+  double pr;
   bool empty;
 };
+// what only the value needs: log sum exp((x - M) / T), log sum exp(x - M), log of the student's mass outside the list
+template <typename C>
+struct RowLogs {
+  C ls, ls1;
+  double log_qr;
+  template <typename Args>
+  __device__ __forceinline__ RowLogs(const Args& a, const RowScal<C>& r, bool two)
+      : ls(lg2(r.S) * (C)LN2), ls1(two ? lg2(r.S1) * (C)LN2 : ls), log_qr((double)(lg2(r.Su) * (C)LN2 + (r.Mu - r.M) * (C)a.invT - ls)) {}
+};
+// u: the unlisted classes, or without an outside class all; l: the listed ones.  Each has its own reference: what the outside class gets is
+// divided among its classes by their softmax, however far below the listed ones they lie.
 template <typename C, typename Args>
-__device__ __forceinline__ RowScal<C> row_scalars(const Args& a, bool tail, bool two, double w, bool has_label, C M, C s_rest, C s_list, C s1,
-                                                  C n_listed, double mass) {
+__device__ __forceinline__ RowScal<C> row_scalars(const Args& a, bool tail, bool two, double w, bool has_label, const Sums<C>& u, const Sums<C>& l, C n_listed,
+                                                  double mass) {
   RowScal<C> r;
-  const C S = tail ? s_rest + s_list : s_rest;
+  r.M = r.Mu = u.m;
+  C S = u.s, S1 = u.s1, wu = C(1), w1 = C(1);
+  if (tail) {
+    const C c = (C)(a.invT * LOG2E);
+    r.M = fmx(u.m, l.m);
+    wu = ex2((u.m - r.M) * c);
+    S = u.s * wu + l.s * ex2((l.m - r.M) * c);
+    if (two) {
+      w1 = ex2((u.m - r.M) * (C)LOG2E);
+      S1 = u.s1 * w1 + l.s1 * ex2((l.m - r.M) * (C)LOG2E);
+    }
+  }
   r.empty = S == C(0);  // every score -inf (the largest score always contributes 1)
-  r.M = M;
-  r.ls = lg2(S) * (C)LN2;
+  r.S = S, r.S1 = S1, r.Su = u.s;
   r.ql = (C)(a.lam * w * a.invT);
   r.qy = has_label ? (C)(a.lab_lam * w) : C(0);
   C rest = C(0);
   r.pr = 0.0;
-  r.log_qr = 0.0;
   if (tail) {
     if ((int64_t)n_listed < a.V) {  // the list may hold every class: then nothing is outside it
       const double left = 1.0 - mass;
       r.pr = left > 0.0 ? left : (left == left ? 0.0 : left);
-      const C qr = s_rest / S;
-      r.log_qr = (double)(lg2(qr) * (C)LN2);
-      rest = (r.pr > 0.0 && qr > C(0)) ? (C)r.pr / qr : C(0);
+      rest = (r.pr > 0.0 && u.s > C(0)) ? (C)r.pr / u.s : C(0);
     }
   }
-  const C total = (C)(mass + r.pr);
-  r.cB = r.ql * total / S;
-  r.cR = tail ? r.ql * (total - rest) / S : r.cB;
-  r.c1 = C(0);
-  r.ls1 = r.ls;
+  const C total = (C)(mass + r.pr), inv = C(1) / S;
+  r.cB = r.ql * total * inv;
+  r.cR = tail ? r.ql * (total * wu * inv - rest) : r.cB;
+  r.c1 = r.c1u = C(0);
   if (two) {
-    r.c1 = r.qy / s1;
-    r.ls1 = lg2(s1) * (C)LN2;
+    r.c1 = r.qy / S1;
+    r.c1u = r.c1 * w1;
   } else {  // labels at T = 1 share e
-    r.cB += r.qy / S;
-    r.cR += r.qy / S;
+    r.cB += r.qy * inv;
+    r.cR += r.qy * wu * inv;
   }
   if (r.empty) {
-    r.cB = r.cR = r.c1 = r.ql = r.qy = C(0);
-    r.M = Lim<C>::lowest;
+    r.cB = r.cR = r.c1 = r.c1u = r.ql = r.qy = C(0);
+    r.M = r.Mu = Lim<C>::lowest;
   }
   return r;
+}
+// the gradient's entry at a listed class (less its teacher's mass and label), and at any other
+template <bool two, typename C>
+__device__ __forceinline__ C entry_listed(const RowScal<C>& r, C x, C c) {
+  return ex2((x - r.M) * c) * r.cB + (two ? ex2((x - r.M) * (C)LOG2E) * r.c1 : C(0));
+}
+template <bool two, typename C>
+__device__ __forceinline__ C entry_other(const RowScal<C>& r, C x, C c) {
+  return ex2((x - r.Mu) * c) * r.cR + (two ? ex2((x - r.Mu) * (C)LOG2E) * r.c1u : C(0));
 }
 
 // probability of a listed entry: log p and p
@@ -144,48 +176,44 @@ __device__ __forceinline__ void power(int squares, const C (&x)[N], const C (&e)
     for (int i = 0; i < N; ++i) what(i, ex2((x[i] - m) * (C)LOG2E));
   }
 }
-// e[i] = 0 where bit i is clear (two operations each; written in C they become a test, a comparison and a choice)
+// f[i] = -inf where bit i is set: two operations each (written in C they become five, or a test, a comparison and a choice)
 template <int I = 0, int N>
-__device__ __forceinline__ void keep(float (&e)[N], unsigned bits) {
+__device__ __forceinline__ void leave_out(float (&f)[N], unsigned bits) {
   if constexpr (I < N) {
     int m;
-    asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(m) : "v"(bits), "n"(I));
-    e[I] = __builtin_bit_cast(float, __builtin_bit_cast(int, e[I]) & m);
-    keep<I + 1>(e, bits);
+    asm("v_bfe_i32 %0, %2, %3, 1\n\tv_bfi_b32 %1, %0, %4, %1" : "=&v"(m), "+v"(f[I]) : "v"(bits), "n"(I), "s"(0xff800000u));
+    leave_out<I + 1>(f, bits);
   }
 }
 template <int N>
-__device__ __forceinline__ void keep(double (&e)[N], unsigned bits) {
+__device__ __forceinline__ void leave_out(double (&f)[N], unsigned bits) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) e[i] = (bits >> i) & 1u ? e[i] : 0.0;
+  for (int i = 0; i < N; ++i) f[i] = (bits >> i) & 1u ? -(double)INFINITY : f[i];
 }
 
 // Sums of one thread, relative to a reference score m that is one of the row's (or the type's lowest value while there is
 // none): any score will do that is not far below the largest, so m is raised rarely, by a branch.  Far:
 // an exponent of 20, whose rounding is 20 * 2^-24 of its exponential, like those of the terms that count least.
-template <typename C, bool TAIL, bool TWO>
-struct Run {
-  C m = Lim<C>::lowest, lim = Lim<C>::lowest, s = C(0), sl = C(0), s1 = C(0), n = C(0);
+template <typename C, bool TWO>
+struct Run : Sums<C> {
+  using Sums<C>::m;
+  using Sums<C>::s;
+  using Sums<C>::s1;
+  C lim = Lim<C>::lowest;
   C c, head;  // log2(e) / T; an exponent of 20 in scores
   int squares;
-  __device__ __forceinline__ Run(double invT, int sq) : c(uniform((C)(invT * LOG2E))), head(uniform((C)(20.0 / fmax(invT, 1.0)))), squares(sq) {}
+  __device__ __forceinline__ Run(double invT, int sq) : Sums<C>(Sums<C>::none()), c(uniform((C)(invT * LOG2E))), head(uniform((C)(20.0 / fmax(invT, 1.0)))), squares(sq) {}
   __device__ __forceinline__ void raise(C to) {
     const C d = m - to;
-    const C f = ex2(d * c);
-    s *= f;
-    if constexpr (TAIL) sl *= f;
+    s *= ex2(d * c);
     if constexpr (TWO) s1 *= ex2(d * (C)LOG2E);
     m = to;
     lim = to + head;
     opaque(m);  // keep the branch
   }
-  __device__ __forceinline__ void listed(C x) {  // a listed class (TAIL only)
-    if (x > lim) raise(x);
-    sl += ex2((x - m) * c);
-    n += C(1);
-  }
   template <int N>
-  __device__ __forceinline__ void add(const C (&f)[N], unsigned bits) {
+  __device__ __forceinline__ void add(C (&f)[N], unsigned bits) {  // bits: elements to leave out
+    if (bits) leave_out(f, bits);
     C vm = f[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) vm = fmx(vm, f[i]);
@@ -198,21 +226,34 @@ struct Run {
       power(squares, f, e, m, [&](int i, C v) { t[i & 1] += v; });
       s1 += t[0] + t[1];
     }
-    if constexpr (TAIL) {
-      if (bits) keep(e, ~bits);
-    }
 #pragma unroll
     for (int o = 1; o < N; o *= 2)
 #pragma unroll
       for (int i = 0; i < N; i += 2 * o) e[i] += e[i + o];
     s += e[0];
   }
-  __device__ __forceinline__ void add1(C x, bool in_list) {
+  __device__ __forceinline__ void add1(C x) {
     if (x > lim) raise(x);
-    if (!(TAIL && in_list)) s += ex2((x - m) * c);
+    s += ex2((x - m) * c);
     if constexpr (TWO) s1 += ex2((x - m) * (C)LOG2E);
   }
+  // over the wave's lanes
+  __device__ __forceinline__ Sums<C> joined() const {
+    Sums<C> o = Sums<C>::none();
+    o.m = wave_max(m);
+    o.s = wave_sum(s * ex2((m - o.m) * c));
+    if constexpr (TWO) o.s1 = wave_sum(s1 * ex2((m - o.m) * (C)LOG2E));
+    return o;
+  }
 };
+// of two sets of scores
+template <bool TWO, typename C>
+__device__ __forceinline__ void join(Sums<C>& to, const Sums<C>& o, C c) {
+  const C m = fmx(to.m, o.m), d = to.m - m, e = o.m - m;
+  to.s = to.s * ex2(d * c) + o.s * ex2(e * c);
+  if constexpr (TWO) to.s1 = to.s1 * ex2(d * (C)LOG2E) + o.s1 * ex2(e * (C)LOG2E);
+  to.m = m;
+}
 
 // ---- the general form: a row in parts, two reads ------------------------------------------------------------------
 // Any length, and few rows: a part per workgroup.  First launch: the statistics of each part (and the listed scores, which an
@@ -246,7 +287,9 @@ __global__ __launch_bounds__(PT) void distill_part_stats(DArgs a) {
   using C = typename Elem<T>::C;
   constexpr int N = Elem<T>::N;
   extern __shared__ unsigned bm[];
-  __shared__ C sm[PT / 64][5];
+  __shared__ Sums<C> sm[PT / 64][2];
+  __shared__ C sn[PT / 64];
+  __shared__ int dup;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Part<T> q(a);
   if (a.w != nullptr && ld_real_u(a.w, a.wdt, q.row) == 0.0) return;
@@ -261,9 +304,11 @@ __global__ __launch_bounds__(PT) void distill_part_stats(DArgs a) {
   const T edge = q.ee >= 0 ? xr[q.ee] : (T)0.f;
   if constexpr (TAIL) {
     for (int i = tid; i < q.words; i += PT) bm[i] = 0;
+    if (tid == 0) dup = 0;
     __syncthreads();
   }
-  Run<C, TAIL, TWO> run(a.invT, a.squares);
+  Run<C, TWO> run(a.invT, a.squares), list(a.invT, a.squares);
+  C n = C(0);  // listed classes
   bool bad = false;
   for (int k = tid; k < a.K; k += PT) {
     const int64_t id = ld_int(a.idx, a.ibits, q.row * a.ldi + k);
@@ -274,7 +319,8 @@ __global__ __launch_bounds__(PT) void distill_part_stats(DArgs a) {
       if constexpr (TAIL) {
         const int b = (int)id - q.bbase;
         const unsigned old = atomicOr(&bm[b >> 5], 1u << (b & 31));
-        if (!((old >> (b & 31)) & 1u)) run.listed(x);
+        if (!((old >> (b & 31)) & 1u)) list.add1(x), n += C(1);
+        else dup = 1;
       }
     }
   }
@@ -283,7 +329,19 @@ __global__ __launch_bounds__(PT) void distill_part_stats(DArgs a) {
     bad |= y < -1 || y >= a.V;
     if (q.has(y)) a.xk[q.r * (a.K + 1) + a.K] = (double)up<T>(xr[y]);
   }
-  if constexpr (TAIL) __syncthreads();
+  if constexpr (TAIL) {
+    __syncthreads();
+    if (dup) {  // a class listed twice: its first entry counts, whichever came to the bitmap first, so that the sums keep their order
+      list = Run<C, TWO>(a.invT, a.squares), n = C(0);
+      for (int k = tid; k < a.K; k += PT) {
+        const int64_t id = ld_int(a.idx, a.ibits, q.row * a.ldi + k);
+        if (!q.has(id)) continue;
+        bool first = true;
+        for (int o = 0; o < k; ++o) first &= ld_int(a.idx, a.ibits, q.row * a.ldi + o) != id;
+        if (first) list.add1(up<T>(xr[id])), n += C(1);
+      }
+    }
+  }
   for (int v = q.v0 + tid; v - tid < q.v1; v += PV * PT) {
     if (v != q.v0 + tid) load(v);
 #pragma unroll
@@ -295,29 +353,24 @@ __global__ __launch_bounds__(PT) void distill_part_stats(DArgs a) {
   }
   if (q.ee >= 0) {
     const int b = q.ee - q.bbase;
-    run.add1(up<T>(edge), TAIL && ((bm[b >> 5] >> (b & 31)) & 1u));
+    if (!(TAIL && ((bm[b >> 5] >> (b & 31)) & 1u))) run.add1(up<T>(edge));
   }
   if (bad) run.s = (C)NAN;
-  const C M = wave_max(run.m);
-  const C f = ex2((run.m - M) * run.c);
-  const C s = wave_sum(run.s * f), sl = TAIL ? wave_sum(run.sl * f) : C(0), n = TAIL ? wave_sum(run.n) : C(0);
-  const C s1 = TWO ? wave_sum(run.s1 * ex2((run.m - M) * (C)LOG2E)) : C(0);
-  if (lane == 0) sm[wave][0] = M, sm[wave][1] = s, sm[wave][2] = sl, sm[wave][3] = s1, sm[wave][4] = n;
+  const Sums<C> u = run.joined();
+  Sums<C> l = Sums<C>::none();
+  if constexpr (TAIL) l = list.joined(), n = wave_sum(n);
+  if (lane == 0) sm[wave][0] = u, sm[wave][1] = l, sn[wave] = n;
   __syncthreads();
   if (tid == 0) {
-    C m = sm[0][0];
-    for (int i = 1; i < PT / 64; ++i) m = fmx(m, sm[i][0]);
-    C o[4] = {};
-    for (int i = 0; i < PT / 64; ++i) {
-      const C g = ex2((sm[i][0] - m) * run.c);
-      o[0] += sm[i][1] * g;
-      o[1] += sm[i][2] * g;
-      if constexpr (TWO) o[2] += sm[i][3] * ex2((sm[i][0] - m) * (C)LOG2E);
-      o[3] += sm[i][4];
+    Sums<C> all = sm[0][0], listed = sm[0][1];
+    n = sn[0];
+    for (int i = 1; i < PT / 64; ++i) {
+      join<TWO>(all, sm[i][0], run.c);
+      if constexpr (TAIL) join<TWO>(listed, sm[i][1], run.c), n += sn[i];
     }
     double* st = a.stat + (q.r * a.parts + q.part) * STAT;
-    st[0] = (double)m;
-    for (int i = 0; i < 4; ++i) st[1 + i] = (double)o[i];
+    st[0] = (double)all.m, st[1] = (double)all.s, st[2] = (double)all.s1;
+    st[3] = (double)listed.m, st[4] = (double)listed.s, st[5] = (double)listed.s1, st[6] = (double)n;
   }
 }
 
@@ -350,8 +403,12 @@ __global__ __launch_bounds__(PT) void distill_part_grad(DArgs a) {
     // the row's parts, one lane each
     const double* st = a.stat + q.r * a.parts * STAT;
     const int mine = min(lane, a.parts - 1) * STAT;
-    const C pm = (C)st[mine], ps = (C)st[mine + 1], pl = TAIL ? (C)st[mine + 2] : C(0), p1 = TWO ? (C)st[mine + 3] : C(0),
-            pn = TAIL ? (C)st[mine + 4] : C(0);
+    Sums<C> pu = Sums<C>::none(), pl = pu;
+    C pn = C(0);
+    pu.m = (C)st[mine], pu.s = (C)st[mine + 1];
+    if constexpr (TWO) pu.s1 = (C)st[mine + 2];
+    if constexpr (TAIL) pl.m = (C)st[mine + 3], pl.s = (C)st[mine + 4], pn = (C)st[mine + 6];
+    if constexpr (TAIL && TWO) pl.s1 = (C)st[mine + 5];
     load(q.v0 + tid);
     const T edge = q.ee >= 0 ? xr[q.ee] : (T)0.f;
     for (int i = tid; i < q.words; i += PT) bm[i] = 0;
@@ -404,13 +461,20 @@ __global__ __launch_bounds__(PT) void distill_part_grad(DArgs a) {
       mass = ts == C(0) ? 0.0 : (double)(ts / ts);  // a list without mass: no teacher
     }
     const bool in = lane < a.parts;
-    const C M = wave_max(pm);
     const C c = (C)(a.invT * LOG2E);
-    const C f = ex2((pm - M) * c);
-    const C s = wave_sum(in ? ps * f : C(0)), sl = TAIL ? wave_sum(in ? pl * f : C(0)) : C(0), nl = TAIL ? wave_sum(in ? pn : C(0)) : C(0);
-    const C s1 = TWO ? wave_sum(in ? p1 * ex2((pm - M) * (C)LOG2E) : C(0)) : C(0);
-    const RowScal<C> rs = row_scalars<C>(a, TAIL, TWO, w, y >= 0, M, s, sl, s1, nl, mass);
-    auto entry = [&](C x, C coef) { return ex2((x - rs.M) * c) * coef + (TWO ? ex2((x - rs.M) * (C)LOG2E) * rs.c1 : C(0)); };
+    auto over_parts = [&](const Sums<C>& p) {
+      Sums<C> o = Sums<C>::none();
+      o.m = wave_max(p.m);
+      o.s = wave_sum(in ? p.s * ex2((p.m - o.m) * c) : C(0));
+      if constexpr (TWO) o.s1 = wave_sum(in ? p.s1 * ex2((p.m - o.m) * (C)LOG2E) : C(0));
+      return o;
+    };
+    const Sums<C> u = over_parts(pu);
+    Sums<C> l = Sums<C>::none();
+    C nl = C(0);
+    if constexpr (TAIL) l = over_parts(pl), nl = wave_sum(in ? pn : C(0));
+    const RowScal<C> rs = row_scalars<C>(a, TAIL, TWO, w, y >= 0, u, l, nl, mass);
+    const RowLogs<C> lg(a, rs, TWO);
     for (int v = q.v0 + tid; v - tid < q.v1; v += PV * PT) {
       if (v != q.v0 + tid) load(v);
 #pragma unroll
@@ -419,11 +483,11 @@ __global__ __launch_bounds__(PT) void distill_part_grad(DArgs a) {
         C x[N], o[N];
         unpack<T>(d[j], x);
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = entry(x[i], rs.cR);
+        for (int i = 0; i < N; ++i) o[i] = entry_other<TWO>(rs, x[i], c);
         st16(at16(gm, v + j * PT), pack<T>(o));
       }
     }
-    if (q.ee >= 0) gr[q.ee] = (T)entry(up<T>(edge), rs.cR);
+    if (q.ee >= 0) gr[q.ee] = (T)entry_other<TWO>(rs, up<T>(edge), c);
     __syncthreads();  // the vectors are written: the listed entries go over them
     const double* xk = a.xk + q.r * (a.K + 1);
     for (int k = tid; k < a.K; k += PT) {
@@ -432,7 +496,7 @@ __global__ __launch_bounds__(PT) void distill_part_grad(DArgs a) {
       C lp, p;
       entry_p<C>(a, q.row, k, norm, lp, p);
       const C x = (C)xk[k];
-      if (q.part == 0 && !rs.empty && p != C(0) && a.lam != 0.0) v_row += a.lam * w * (double)(p * (lp - ((x - rs.M) * (C)a.invT - rs.ls)));
+      if (q.part == 0 && !rs.empty && p != C(0) && a.lam != 0.0) v_row += a.lam * w * ((double)p * ((double)lp - ((double)(x - rs.M) * a.invT - (double)lg.ls)));
       if (q.has(id)) {
         C ph = p;
         bool owner = true;
@@ -445,19 +509,19 @@ __global__ __launch_bounds__(PT) void distill_part_grad(DArgs a) {
             ph += po;
           }
         }
-        if (owner) gr[id] = (T)(entry(x, rs.cB) - rs.ql * ph - (id == y ? rs.qy : C(0)));
+        if (owner) gr[id] = (T)(entry_listed<TWO>(rs, x, c) - rs.ql * ph - (id == y ? rs.qy : C(0)));
       }
     }
     if (tid == PT - 1) {
       if (q.has(y)) {
         const int b = (int)y - q.bbase;
-        if (!((bm[b >> 5] >> (b & 31)) & 1u)) gr[y] = (T)(entry((C)xk[a.K], rs.cR) - rs.qy);
+        if (!((bm[b >> 5] >> (b & 31)) & 1u)) gr[y] = (T)(entry_other<TWO>(rs, (C)xk[a.K], c) - rs.qy);
       }
       if (q.part == 0 && !rs.empty) {
-        if (TAIL && rs.pr != 0.0 && a.lam != 0.0) v_row += a.lam * w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - rs.log_qr);
-        if (y >= 0 && y < a.V && a.lab_lam != 0.0) v_row += a.lab_lam * w * (double)(rs.ls1 - ((C)xk[a.K] - rs.M));
+        if (TAIL && rs.pr != 0.0 && a.lam != 0.0) v_row += a.lam * w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - lg.log_qr);
+        if (y >= 0 && y < a.V && a.lab_lam != 0.0) v_row += a.lab_lam * w * (double)(lg.ls1 - ((C)xk[a.K] - rs.M));
       }
-      if (rs.ls != rs.ls) v_row = NAN;  // a NaN score, or an index or label out of range
+      if (rs.S != rs.S) v_row = NAN;  // a NaN score, or an index or label out of range
     }
   }
   if (q.part != 0) return;  // the first part of each row carries its value
@@ -524,7 +588,9 @@ struct RowsGeom {
 };
 
 template <typename T, int NT, int NV, bool tail, bool two>
-__global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) {
+__global__ __launch_bounds__((NT < 256 ? 256 : NT), sizeof(T) == 8 ? 2 : 4) void distill_rows(DArgs) {
+  // (Float64 in 128 registers spills some eighty of them: two waves to a SIMD, and no workgroup of 1024 threads)
+
   // The arguments stay in memory and are read where they are used: hoisted out of the row loop they fill the scalar registers and
   // spill into vector ones
   const PG_CONST_AS DArgs* ap = (const PG_CONST_AS DArgs*)__builtin_amdgcn_kernarg_segment_ptr();
@@ -535,8 +601,9 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
   constexpr int N = G::N, NW = G::NW, GPW = G::GPW;
   constexpr int AGAIN = 1 << 30;  // marks a list entry whose class an earlier one holds
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  __shared__ C sm[GPW][NW][7];
-  __shared__ double smt[GPW][NW];
+  __shared__ Sums<C> sm[NW][2];  // [wave][unlisted, listed]; without an outside class the latter has the teacher's maximum and sum
+  __shared__ C smn[NW];
+  __shared__ double smt[NW];
   __shared__ C sxy[GPW][2];
   __shared__ int flags[GPW][3][2];  // [row mod 3][a class is listed twice, the label is listed]
   const int tid = threadIdx.x % NT, lane = threadIdx.x & 63;
@@ -621,6 +688,20 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     }
     if (tid == NT - 1) sxy[grp][par] = up<T>(xy);
   };
+  // of the entries of one class the first holds it, whichever came to the bitmap first: the sums keep their order
+  auto order_list = [&](int par, int slot) {
+    if (flags[grp][slot][0] == 0) return;
+    int* li = li0 + par * K;
+#pragma clang loop unroll(disable)
+    for (int k = tid; k < K; k += NT) {
+      if (li[k] < 0) continue;
+      const int id = li[k] & ~AGAIN;
+      bool again = false;
+#pragma clang loop unroll(disable)
+      for (int q = 0; q < k; ++q) again |= (li[q] & ~AGAIN) == id;
+      li[k] = again ? id | AGAIN : id;
+    }
+  };
   // head elements: threads 0 ..; tail elements: threads NT - 1 .. down
   auto edge_of = [&](const P& pl) { return tid < pl.h ? tid : (pl.hV + (NT - 1 - tid) < a.V ? pl.hV + (NT - 1 - tid) : -1); };
 
@@ -650,6 +731,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     }
     put_list(row, id, t, y, x, xy, 0, 0);
     group_sync<NT>();
+    order_list(0, 0);
   }
   double v_acc = 0.0;
   while (row < a.nrows) {
@@ -670,9 +752,10 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     ask_list(nrow, id_raw, t_next, y_raw);
 
     // pass 1
-    Run<C, tail, two> run(a.invT, a.squares);
-    // the list, while the row is on its way: the teacher's maximum and sum, the scores that the sums below leave out
-    C tm = Lim<C>::lowest, ts = C(0);
+    Run<C, two> run(a.invT, a.squares);
+    // the list, while the row is on its way: the teacher's mass, or maximum and sum, and the scores that the sums below leave out
+    Run<C, two> listed(a.invT, a.squares);
+    C tm = Lim<C>::lowest, ts = C(0), nl = C(0);
     double tmass = 0.0;
     bool bad = y == -2;
     const double lse = tail ? ld_real_u(a.lse, a.lsedt, row) : 0.0;
@@ -682,7 +765,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
       bad |= id == -2;
       if (id < 0) continue;
       if constexpr (tail) {
-        if (!(id & AGAIN)) run.listed(lx[k]);
+        if (!(id & AGAIN)) listed.add1(lx[k]), nl += C(1);
         tmass += exp_series((double)lt[k] * a.invT - lse);
       } else {
         const C t = (C)((double)lt[k] * a.invT);
@@ -695,72 +778,71 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     }
     int t0 = tid;
     opaque(t0);
+    auto bits_of = [&](int j) { return tail ? listed_bits<T>(bm, min(j * NT + t0, pl.nmain) * N + G::FRONT) : 0u; };
+    unsigned bits_next = bits_of(0);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (j * NT < pl.nmain) {
+        const unsigned bits = bits_next;
+        if (j + 1 < NV) bits_next = bits_of(j + 1);  // on its way from LDS while this vector is added
         if ((j + 1) * NT > pl.nmain) {
           if (j * NT + t0 >= pl.nmain) d[j] = minus_inf16<T>();
           opaque(d[j]);  // keep the branch: every vector but one is whole
         }
         C f[N];
         unpack<T>(d[j], f);
-        run.template add<N>(f, tail ? listed_bits<T>(bm, min(j * NT + t0, pl.nmain) * N + G::FRONT) : 0u);
+        run.add(f, bits);
       }
     }
     if (ee >= 0) {
       const int b = ee - bbase;
-      run.add1(up<T>(edge), tail && ((bm[b >> 5] >> (b & 31)) & 1u));
+      if (!(tail && ((bm[b >> 5] >> (b & 31)) & 1u))) run.add1(up<T>(edge));
     }
     if (bad) run.s = (C)NAN;
     // joined over the group
-    C M = wave_max(run.m);
-    C f = ex2((run.m - M) * c);
-    C s = wave_sum(run.s * f), sl = C(0), nl = C(0), s1 = C(0);
-    if constexpr (tail) sl = wave_sum(run.sl * f), nl = wave_sum(run.n);
-    if constexpr (two) s1 = wave_sum(run.s1 * ex2((run.m - M) * (C)LOG2E));
+    Sums<C> u = run.joined(), l = Sums<C>::none();
     if (wave * 64 < K) {  // a wave that holds entries
       if constexpr (tail) {
+        l = listed.joined();
+        nl = wave_sum(nl);
         tmass = wave_sum(tmass);
       } else {
-        const C wm = wave_max(tm);
-        ts = wave_sum(ts * ex2((tm - wm) * (C)LOG2E));
-        tm = wm;
+        l.m = wave_max(tm);
+        l.s = wave_sum(ts * ex2((tm - l.m) * (C)LOG2E));
       }
     }
     if constexpr (NW > 1) {
       if (lane == 0) {
-        C* o = sm[0][wave];
-        o[0] = M, o[1] = s, o[2] = sl, o[3] = s1, o[4] = nl, o[5] = tm, o[6] = ts;
-        smt[0][wave] = tmass;
+        sm[wave][0] = u, sm[wave][1] = l;
+        if constexpr (tail) smn[wave] = nl, smt[wave] = tmass;
       }
       __syncthreads();
-      const int q = (lane & 15) % NW;
+      const Sums<C> p = sm[(lane & 15) % NW][0];
       const bool in = (lane & 15) < NW;
-      const C pm = sm[0][q][0];
-      M = row16_max(pm);
-      f = in ? ex2((pm - M) * c) : C(0);
-      s = row16_sum(in ? sm[0][q][1] * f : C(0));
-      if constexpr (tail) sl = row16_sum(in ? sm[0][q][2] * f : C(0)), nl = row16_sum(in ? sm[0][q][4] : C(0));
-      if constexpr (two) s1 = row16_sum(in ? sm[0][q][3] * ex2((pm - M) * (C)LOG2E) : C(0));
-      tm = sm[0][0][5], ts = sm[0][0][6], tmass = smt[0][0];
+      u.m = row16_max(p.m);
+      u.s = row16_sum(in ? p.s * ex2((p.m - u.m) * c) : C(0));
+      if constexpr (two) u.s1 = row16_sum(in ? p.s1 * ex2((p.m - u.m) * (C)LOG2E) : C(0));
+      l = sm[0][1];
+      if constexpr (tail) nl = smn[0], tmass = smt[0];
 #pragma clang loop unroll(disable)
       for (int i = 1; i < NW && i * 64 < K; ++i) {
-        if constexpr (tail) {
-          tmass += smt[0][i];
-        } else {
-          const C om = sm[0][i][5], wm = fmx(tm, om);
-          ts = ts * ex2((tm - wm) * (C)LOG2E) + sm[0][i][6] * ex2((om - wm) * (C)LOG2E);
-          tm = wm;
-        }
+        join<tail && two>(l, sm[i][1], tail ? c : (C)LOG2E);
+        if constexpr (tail) nl += smn[i], tmass += smt[i];
       }
     } else {
       group_sync<NT>();
     }
+    tm = l.m, ts = l.s;
     const double norm = tail ? lse : uniform((double)tm + (double)(lg2(ts) * (C)LN2));
     const double mass = tail ? tmass : (ts == C(0) ? 0.0 : (double)(ts / ts));
-    RowScal<C> rs = row_scalars<C>(a, tail, two, w, y >= 0, M, s, sl, s1, nl, mass);
+    RowScal<C> rs = row_scalars<C>(a, tail, two, w, y >= 0, u, l, nl, mass);
     rs.M = uniform(rs.M), rs.cB = uniform(rs.cB), rs.cR = uniform(rs.cR), rs.c1 = uniform(rs.c1), rs.ql = uniform(rs.ql), rs.qy = uniform(rs.qy);
-    rs.ls = uniform(rs.ls), rs.ls1 = uniform(rs.ls1), rs.pr = uniform(rs.pr), rs.log_qr = uniform(rs.log_qr);
+    if constexpr (tail) {
+      rs.Mu = uniform(rs.Mu), rs.c1u = uniform(rs.c1u);
+    } else {
+      rs.Mu = rs.M, rs.c1u = rs.c1;
+    }
+    rs.S = uniform(rs.S), rs.S1 = uniform(rs.S1), rs.Su = uniform(rs.Su), rs.pr = uniform(rs.pr);
     rs.empty = __builtin_amdgcn_readfirstlane(rs.empty);
     const int slot_next = slot == 2 ? 0 : slot + 1;
     if (tid < 2) flags[grp][slot_next == 2 ? 0 : slot_next + 1][tid] = 0;  // the row before this one is through with them
@@ -778,8 +860,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
     if (more && en >= 0) edge_next = xn[en];
     int off = tid * 16;
     opaque(off);  // NV sums that stay out of the row loop's registers
-    auto entry = [&](C x, C coef) { return ex2((x - rs.M) * c) * coef + (two ? ex2((x - rs.M) * (C)LOG2E) * rs.c1 : C(0)); };
-    // For the two-byte types the coefficient goes into the exponent, |cR| exp2((x - M) c) = exp2((x - M) c + log2 |cR|): an operation
+    // For the two-byte types the coefficient goes into the exponent, |cR| exp2((x - Mu) c) = exp2((x - Mu) c + log2 |cR|): an operation
     // a score less.  The logarithm, 100 at most in earnest, is off by 2^-18: 3e-6 of an entry that is then rounded by up to
     // 2^-12 (Float16) of it.
     const C fold = uniform(lg2((C)fabs(rs.cR)));
@@ -795,14 +876,14 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
         unpack<T>(d[j], x);
         if constexpr (sizeof(T) == 2 && !two) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) o[i] = ex2(fma(x[i] - rs.M, c, fold));
+          for (int i = 0; i < N; ++i) o[i] = ex2(fma(x[i] - rs.Mu, c, fold));
           out = pack<T>(o);
           if constexpr (tail) out ^= u32x4{sign, sign, sign, sign};
         } else {
 #pragma unroll
-          for (int i = 0; i < N; ++i) o[i] = ex2((x[i] - rs.M) * c);
+          for (int i = 0; i < N; ++i) o[i] = ex2((x[i] - rs.Mu) * c);
           if constexpr (two) {
-            power(a.squares, x, o, rs.M, [&](int i, C v) { o[i] = o[i] * rs.cR + v * rs.c1; });
+            power(a.squares, x, o, rs.Mu, [&](int i, C v) { o[i] = o[i] * rs.cR + v * rs.c1u; });
           } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) o[i] *= rs.cR;
@@ -813,8 +894,9 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
       stb16(rg, off + j * NT * 16, out);
       d[j] = ldb16(rn, off + j * NT * 16);
     }
-    if (ee >= 0) gr[ee] = (T)entry(up<T>(edge), rs.cR);
+    if (ee >= 0) gr[ee] = (T)entry_other<two>(rs, up<T>(edge), c);
     asm volatile("" : "+s"(ap));
+    const RowLogs<C> lg(a, rs, two);
     // the list's probabilities and its part of the value; its bits go
 #pragma clang loop unroll(disable)
     for (int k = tid; k < K; k += NT) {
@@ -824,7 +906,7 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
         const double t = (double)lt[k] * a.invT;
         const C l = t == -INFINITY ? (C)t : (C)(t - norm);  // (a list of -inf only has no norm)
         p = ex2(l * (C)LOG2E);
-        if (p != C(0) && !rs.empty && a.lam != 0.0) v_acc += a.lam * w * (double)(p * (l - ((lx[k] - rs.M) * (C)a.invT - rs.ls)));
+        if (p != C(0) && !rs.empty && a.lam != 0.0) v_acc += a.lam * w * ((double)p * ((double)l - ((double)(lx[k] - rs.M) * a.invT - (double)lg.ls)));
         bm[((id & ~AGAIN) - bbase) >> 5] = 0;
       }
       lp[k] = p;
@@ -842,17 +924,18 @@ __global__ __launch_bounds__((NT < 256 ? 256 : NT), 4) void distill_rows(DArgs) 
         for (int q = 0; q < K; ++q)
           if (li[q] == (id | AGAIN)) ph += lp[q];
       }
-      gr[id] = (T)(entry(lx[k], rs.cB) - rs.ql * ph - (id == y ? rs.qy : C(0)));
+      gr[id] = (T)(entry_listed<two>(rs, lx[k], c) - rs.ql * ph - (id == y ? rs.qy : C(0)));
     }
     if (tid == NT - 1) {
       if (y >= 0) {
         const C xy = sxy[grp][par];
-        if (!flags[grp][slot][1]) gr[y] = (T)(entry(xy, rs.cR) - rs.qy);
-        if (!rs.empty && a.lab_lam != 0.0) v_acc += a.lab_lam * w * (double)(rs.ls1 - (xy - rs.M));
+        if (!flags[grp][slot][1]) gr[y] = (T)(entry_other<two>(rs, xy, c) - rs.qy);
+        if (!rs.empty && a.lab_lam != 0.0) v_acc += a.lab_lam * w * (double)(lg.ls1 - (xy - rs.M));
       }
-      if (tail && rs.pr != 0.0 && !rs.empty && a.lam != 0.0) v_acc += a.lam * w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - rs.log_qr);
-      if (rs.ls != rs.ls) v_acc = NAN;  // a NaN score, or an index or label out of range
+      if (tail && rs.pr != 0.0 && !rs.empty && a.lam != 0.0) v_acc += a.lam * w * rs.pr * ((double)(lg2((C)rs.pr) * (C)LN2) - lg.log_qr);
+      if (rs.S != rs.S) v_acc = NAN;  // a NaN score, or an index or label out of range
     }
+    order_list(par ^ 1, slot_next);
     edge = edge_next;
     y = y_next;
     w = w_next;
@@ -905,7 +988,7 @@ pg_status run_mode(pg_ctx* c, const DArgs& a, int64_t rows) {
   PG_ROWS_TRY(256, 8);
   PG_ROWS_TRY(256, 16);
   PG_ROWS_TRY(512, 16);
-  PG_ROWS_TRY(1024, 16);
+  if constexpr (sizeof(T) < 8) PG_ROWS_TRY(1024, 16);
 #undef PG_ROWS_TRY
   return run_parts<T, tail, two>(c, a, rows);
 }

@@ -7,9 +7,10 @@ largest terms and its tree of additions, and a listed entry subtracts a teacher'
 The oracle adds these up per entry (`size`: every term times 64 + 6 |x - m| c, or 64 + 4 |l|), the tests allow size * u.
 
 The hardware's Float32 exponential gives 0 for results below 2^-126.  An entry is a coefficient times such an exponential, of a score
-against one that is no larger than the row's largest, so at most coefficient * 2^-126 is lost; the entry of the largest score is the
-coefficient times 1 or more, its `size` 64 of that or more, hence max(size of the row) / 64 * 2^-126.  Where the coefficient is in the
-exponent (the two-byte types) the loss is 2^-126 itself."""
+against one of the row's that is at most an exponent of 20 below the largest; where listed and other classes have references of
+their own, the coefficient holds the exponential of their distance.  So at most exp(20) * 2^-126 < 2^-97 of the largest score's entry is
+lost, whose `size` is 64 of it or more, hence max(size of the row) / 64 * 2^-97.  Where the coefficient is in the
+exponent (the two-byte types) the loss is 2^-97 itself."""
 import numpy as np
 import pytest
 import torch
@@ -28,7 +29,7 @@ def pa():
 
 
 def flushed(size):
-    return 2.0**-126 * np.maximum(1.0, size.max(axis=1, keepdims=True, initial=0.0) / 64)
+    return 2.0**-97 * np.maximum(1.0, size.max(axis=1, keepdims=True, initial=0.0) / 64)
 
 
 def check(got, value, want, dtype):
