@@ -190,21 +190,20 @@ __device__ __forceinline__ double uniform(double v) { return pg_readlane(v, 0); 
 
 // (one instruction; results below 2^-126 are 0: an exponent of 20 below the largest's, 2^-97 of it)
 __device__ __forceinline__ float ex2(float v) { return __builtin_amdgcn_exp2f(v); }
-__device__ __forceinline__ double ex2(double v) { return exp2(v); }
+__device__ __forceinline__ double ex2(double v);  // below
 __device__ __forceinline__ float lg2(float v) { return __builtin_amdgcn_logf(v); }
 __device__ __forceinline__ double lg2(double v) { return log2(v); }
-// exp(x) in Float64 from its series: x = n ln 2 + r, |r| <= ln(2) / 2, sum of r^k / k! up to k = 12 (the next term is below 2^-52
-// of the sum), times 2^n.  The library's exp inside a loop keeps its constants in some forty vector registers around the
-// loop, which a kernel that holds a row in registers has not got; here they pass through scalar registers where they are used.
+// exp in Float64 from its series: argument n ln 2 + r, |r| <= ln(2) / 2, sum of r^k / k! up to k = 13 (the next term is below 2^-56
+// of the sum), times 2^n.  The library's exp and exp2 inside a loop keep their constants in some forty vector registers around
+// the loop, which a kernel that holds a row in registers has not got: the compiler moved them to and fro, and in one of its
+// builds lanes lost a coefficient on the way (sums off by 1e-11).  Here they pass through scalar registers where they are used.
 __device__ __forceinline__ double scalar_const(double v) {
   asm volatile("" : "+s"(v));
   return v;
 }
-__device__ __forceinline__ double exp_series(double x) {
-  const double n = rint(x * 1.4426950408889634);
-  double r = fma(n, scalar_const(-0x1.62e42fefa38p-1), x);  // ln 2 in two pieces, the first with zeros at its end
-  r = fma(n, scalar_const(-0x1.ef35793c7673p-45), r);
-  double p = scalar_const(1.0 / 479001600.0);
+__device__ __forceinline__ double exp_sum(double r) {
+  double p = scalar_const(1.0 / 6227020800.0);
+  p = fma(p, r, scalar_const(1.0 / 479001600.0));
   p = fma(p, r, scalar_const(1.0 / 39916800.0));
   p = fma(p, r, scalar_const(1.0 / 3628800.0));
   p = fma(p, r, scalar_const(1.0 / 362880.0));
@@ -216,9 +215,18 @@ __device__ __forceinline__ double exp_series(double x) {
   p = fma(p, r, scalar_const(1.0 / 6.0));
   p = fma(p, r, 0.5);
   p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  p = ldexp(p, (int)fmax(fmin(n, 2000.0), -2000.0));
-  return x < -745.2 ? 0.0 : (x > 709.8 ? (double)INFINITY : p);  // (NaN stays NaN)
+  return fma(p, r, 1.0);
+}
+__device__ __forceinline__ double exp_scale(double p, double n) { return ldexp(p, (int)fmax(fmin(n, 2000.0), -2000.0)); }
+__device__ __forceinline__ double exp_series(double x) {
+  const double n = rint(x * 1.4426950408889634);
+  double r = fma(n, scalar_const(-0x1.62e42fefa38p-1), x);  // ln 2 in two pieces, the first with zeros at its end
+  r = fma(n, scalar_const(-0x1.ef35793c7673p-45), r);
+  return x < -745.2 ? 0.0 : (x > 709.8 ? (double)INFINITY : exp_scale(exp_sum(r), n));  // (NaN stays NaN)
+}
+__device__ __forceinline__ double ex2(double x) {
+  const double n = rint(x);
+  return x < -1080.0 ? 0.0 : (x > 1030.0 ? (double)INFINITY : exp_scale(exp_sum((x - n) * scalar_const(0x1.62e42fefa39efp-1)), n));
 }
 
 template <typename C>

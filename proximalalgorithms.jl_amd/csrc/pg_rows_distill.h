@@ -8,8 +8,8 @@
 // the unlisted classes themselves (1 - sum of the listed q loses everything where the student agrees with the teacher),
 // which a bitmap of the row in LDS makes possible; the bitmap also finds classes listed twice.
 //
-// Bound by memory: 8192 x 131072 bf16 835 us (5.15 TB/s read and written, a copy of that size 4.7), 4096 x 32768 bf16 103 us (5.2; a copy 5.4);
-// with the outside class, 2048 x 131000 bf16, 248 us (4.3): 31 us a row and CU, 25 of them memory, the vector unit 19 (half of
+// Bound by memory: 8192 x 131072 bf16 838 us (5.13 TB/s read and written, a copy of that size 4.7), 4096 x 32768 bf16 103 us (5.2; a copy 5.4);
+// with the outside class, 2048 x 131000 bf16, 250 us (4.3): 31 us a row and CU, 25 of them memory, the vector unit 19 (half of
 // that two exponentials a score at a quarter of the rate) -- the difference is the reduction between the passes.
 #pragma once
 #include <algorithm>

@@ -386,6 +386,49 @@ def test_masked_classes_and_terms_that_are_switched_off(dtype, n, v):
             check(g, val, want, DT[dtype])
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n,v", [(6, 300), (2, 70000), (300, 5000)])
+@pytest.mark.parametrize("below", [60.0, 200.0, 5000.0])
+def test_outside_class_far_below_the_listed_ones(dtype, n, v, below):
+    """what the teacher leaves outside its list is divided by the softmax of the other classes, also where they have no share of the whole row's"""
+    rng = np.random.default_rng(int(below))
+    base = min(n, 4)
+    t, idx = teacher(rng, base, v, 7)
+    x, _ = scores(rng, base, v, DT[dtype])
+    x.scatter_add_(1, torch.from_numpy(idx).cuda(), torch.full((base, 7), below, dtype=x.dtype, device="cuda"))
+    xe = x.double().cpu().numpy()
+    td, te = tdev(t, torch.float32)
+    lse = np.log(np.exp(te / 2).sum(1) * 1.3).astype(np.float32)
+    y = rng.integers(0, v, base)
+    each = repeated(n, base)
+    kw = dict(temperature=2.0, lam=1.5, label_lam=0.5)
+    f = pa().DistillationLoss(td[each], torch.from_numpy(idx).cuda()[each], v, teacher_lse=torch.from_numpy(lse).cuda()[each], labels=torch.from_numpy(y).cuda()[each], **kw)
+    val, g = f.value_and_gradient(x[each])
+    alone = [ref.distillation(xe[b:b + 1], te[b:b + 1], idx[b:b + 1], teacher_lse=lse[b:b + 1].astype(np.float64), labels=y[b:b + 1], **kw) for b in range(base)]
+    assert all(np.isfinite(w[0]) and (w[1] < 0).any() for w in alone)
+    check_repeated(g, val, ((None, np.concatenate([w[1] for w in alone]), np.concatenate([w[2] for w in alone]), None), alone), DT[dtype], n)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n,v,k", [(200, 900, 300), (70, 30000, 200), (2, 70000, 300)])
+@pytest.mark.parametrize("rest", [False, True])
+def test_classes_listed_many_times_give_the_same_bits_each_time(dtype, n, v, k, rest):
+    rng = np.random.default_rng(k)
+    t, idx = teacher(rng, n, v, k)
+    idx[:, k // 3:] = idx[:, rng.integers(0, k // 3, k - k // 3)]  # three entries to a class on average
+    td, te = tdev(t, torch.float32)
+    x, xe = scores(rng, n, v, DT[dtype], idx, t)
+    lse = np.log(np.exp(te).sum(1) * 1.2)
+    f = pa().DistillationLoss(td, torch.from_numpy(idx).cuda(), v, teacher_lse=torch.from_numpy(lse).cuda() if rest else None)
+    val, g = f.value_and_gradient(x)
+    for _ in range(8):
+        v2, g2 = f.value_and_gradient(x)
+        assert v2 == val and torch.equal(g2, g)
+    rows = [0, n - 1]
+    want = ref.distillation(xe[rows], te[rows], idx[rows], teacher_lse=lse[rows] if rest else None)
+    check(g[rows], want[0], want, DT[dtype])
+
+
 def test_balance_of_nothing_and_positions_on_the_device():
     m = pa()
     for offsets in (None, [0], [0, 0, 0]):
