@@ -571,8 +571,9 @@ pg_status run_parts(pg_ctx* c, DArgs a, int64_t rows) {
 // registers and, as a vector leaves, loads the same vector of the group's NEXT row in its place, so that the memory pipes
 // stay busy through the reduction.  Loads return in order, so nothing may be asked for between those loads and pass 1 that
 // is needed before it: the next row's list is asked for a pass ahead and waits in LDS, and no register may spill there.
-// A workgroup's vectors start at a 128-byte line of the scores, and of the gradient where its rows lie alike, or each wave's
-// access ends in two half lines (2048 x 131000 bf16: both on a line 235 us, one of them 246, both 8 bytes off 257).
+// Vectors start at a 128-byte line of the scores, and of the gradient where its rows lie alike, or each wave's access ends in two half
+// lines (2048 x 131000 bf16: both on a line 235 us, one of them 246, both 8 bytes off 257; 65536 x 1003 f32, a wave to a row,
+// 105 against 114 with vectors from 16 bytes).  64 bytes for a wave's rows of two-byte types: head and tail take a thread each.
 template <typename T, int NT, int NV>
 struct RowsGeom {
   using C = typename Elem<T>::C;
@@ -580,8 +581,8 @@ struct RowsGeom {
   static constexpr int WG = NT < 256 ? 256 : NT;
   static constexpr int GPW = WG / NT, NW = NT / 64;
   static constexpr int capacity = NT * NV * N;  // classes a group's registers hold
-  static constexpr int ALIGN = NT == 64 ? 16 : 128;
-  static constexpr int FRONT = NT == 64 ? BIT0 : 64;  // bits in front of the first vector's: at least its head
+  static constexpr int ALIGN = NT == 64 && sizeof(T) == 2 ? 64 : 128;
+  static constexpr int FRONT = NT == 64 ? 32 : 64;  // bits in front of the first vector's: at least its head
   static __host__ __device__ int words(int V) { return ((V + FRONT + N + 31) / 32 + 1) & ~1; }
   // two bitmaps and two lists (this row's, the next's) of scores and classes, one of logits and of probabilities
   static __host__ __device__ int group_bytes(int V, int K) { return words(V) * 8 + (K * (4 * (int)sizeof(C) + 8) + 7) / 8 * 8; }
