@@ -429,6 +429,56 @@ def test_classes_listed_many_times_give_the_same_bits_each_time(dtype, n, v, k, 
     check(g[rows], want[0], want, DT[dtype])
 
 
+@pytest.mark.parametrize("dtype,logits,n,v,k", [("f32", "f32", 150, 70000, 1024), ("bf16", "f64", 2000, 100, 50), ("f64", "f32", 1500, 40, 33), ("f16", "f16", 200, 140001, 700)])
+@pytest.mark.parametrize("rest", [False, True])
+def test_parts_of_more_rows_than_the_workspace_holds(dtype, logits, n, v, k, rest):
+    rng = np.random.default_rng(n)
+    base = 5
+    t, idx = teacher(rng, base, v, k, absent=0.05)
+    td, te = tdev(t, DT[logits])
+    x, xe = scores(rng, base, v, DT[dtype], idx, t)
+    lse = np.log(np.where(idx >= 0, np.exp(te), 0).sum(1) * 1.2)
+    each = repeated(n, base)
+    f = pa().DistillationLoss(td[each], torch.from_numpy(idx).cuda()[each], v, teacher_lse=torch.from_numpy(lse).cuda()[each] if rest else None)
+    val, g = f.value_and_gradient(x[each])
+    alone = [ref.distillation(xe[b:b + 1], te[b:b + 1], idx[b:b + 1], teacher_lse=lse[b:b + 1] if rest else None) for b in range(base)]
+    check_repeated(g, val, ((None, np.concatenate([w[1] for w in alone]), np.concatenate([w[2] for w in alone]), None), alone), DT[dtype], n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shift", [0, 3])
+def test_the_longest_row(dtype, shift):
+    """2^24 classes, against the formula in Float64 on the device"""
+    v = 1 << 24
+    gen = torch.Generator("cuda").manual_seed(1)
+    x = torch.empty(v + shift, device="cuda", dtype=DT[dtype])[shift:].view(1, v)
+    x.copy_(torch.randn(1, v, device="cuda", generator=gen))
+    idx = torch.tensor([[0, 1, v - 1, v // 2]], device="cuda")
+    t = torch.tensor([[3.0, 2.0, 1.0, 0.0]], device="cuda")
+    x[0, idx[0]] = 18.0
+    f = pa().DistillationLoss(t, idx, v)
+    val, g = f.value_and_gradient(x)
+    p, lq = torch.softmax(t.double(), 1), torch.log_softmax(x.double(), 1)
+    want = lq.exp()
+    want[0, idx[0]] -= p[0]
+    # a thread adds 128 vectors one after another: 128 roundings of the sum beside the 64 + 6 |x - m| log2(e), |x - m| < 25, of the others
+    tol = want.abs() * torch.finfo(x.dtype).eps / 2 + lq.exp() * 2.0**-24 * (128 + 64 + 6 * 36) + 2.0**-97
+    tol[0, idx[0]] += 2.0**-24 * 64  # the teacher's probabilities
+    assert bool(((g.double() - want).abs() <= tol).all())
+    kl = float((p * (p.log() - lq[0, idx[0]])).sum())
+    assert abs(val - kl) <= 2.0**-24 * 64 * 40
+
+
+def test_balance_of_very_many_groups():
+    rng = np.random.default_rng(0)
+    n, e, k = 20000, 8, 2
+    x, xe = router(rng, n, e, torch.float32)
+    for offsets in (list(range(n + 1)), sorted([0, n, *rng.integers(0, n, 3000).tolist()])):
+        loss = pa().BalanceLoss(n, e, k, offsets=offsets)
+        val, g = loss.value_and_gradient(x)
+        check_balance(loss, g, val, ref.balance(xe, k, offsets=offsets), torch.float32)
+
+
 def test_balance_of_nothing_and_positions_on_the_device():
     m = pa()
     for offsets in (None, [0], [0, 0, 0]):
