@@ -8,12 +8,12 @@
 // L lanes take a token, 64 / L tokens a wave: lane l of them holds, in chunk i, the V experts from (i L + l) V on (16 bytes, so that a
 // token's chunk is read in one piece).  The k-th highest score is found by bisection over the scores' bit patterns, mapped to
 // unsigned numbers in the scores' order: a step counts the keys from a threshold on, whatever k is, all tokens of the wave
-// at once, and starts from the thresholds of the wave's tokens before.  (With a token per wave the search runs in scalar
+// at once, and starts from the thresholds of the wave's tokens before (the first ones from the normal distribution's).  (With a token per wave the search runs in scalar
 // registers, on the one scalar unit the CU has: 80 us for 131072 x 256 against 46 with four tokens in vector ones.)
 //
 // 131072 x 256 f32 (134 MB read twice, 134 written): 94 us, the counting 46 -- 33 with a single step of the search, 7.5 steps of 48
 // operations on average --, the gradients 47, 5.7 TB/s.  Small calls are launches and the search of a wave's first tokens: 16384 x 128
-// bf16 9 + 9 us, 6 + 9 with a single step.
+// bf16 8 + 8.5 us, 6 of the 8 with a single step.
 #include <algorithm>
 
 #include "pg_rows.h"
@@ -34,6 +34,7 @@ struct BArgs {
   unsigned copies;  // of a group's accumulator, taken in turn by its tiles: atomics to one line wait for each other
   int E, k, cbits;
   double lam_e_k;  // lam * experts / k
+  float z;         // where a normal distribution has k / experts above
   double *partials, *out;
   unsigned* counter;
   void* value;
@@ -237,6 +238,26 @@ __device__ __forceinline__ pg_balance_tile tile_at(const BArgs& a, int64_t q) {
   return t;
 }
 
+// a threshold for a wave's first tokens to start from: where a normal distribution of the token's mean and variance has k experts above.
+// From there the search takes 6 steps, from a fixed number 10; this takes two steps' time (16384 x 128 bf16 in turn 17.1 us against 18.2).
+template <typename T, int L, int NI>
+__device__ __forceinline__ typename Key<T>::U first_guess(const T (&x)[Geom<T, L, NI>::PL], float z) {
+  float n = 0.f, sum = 0.f, sq = 0.f;
+#pragma unroll
+  for (int i = 0; i < Geom<T, L, NI>::PL; ++i) {
+    const float f = (float)x[i];
+    const bool in = f > -INFINITY;
+    n += in ? 1.f : 0.f;
+    const float v = in ? f : 0.f;
+    sum += v;
+    sq = fma(v, v, sq);
+  }
+  n = token_sum<L>(n), sum = token_sum<L>(sum), sq = token_sum<L>(sq);
+  const float inv = __builtin_amdgcn_rcpf(n), mean = sum * inv;
+  const typename Key<T>::U g = Key<T>::of((T)(mean + z * __builtin_amdgcn_sqrtf(fmaxf(sq * inv - mean * mean, 0.f))));
+  return g > 1 ? g : Key<T>::of((T)1.0f);  // (no scores, or infinite ones)
+}
+
 // choices of the tokens [t0, t1) into sc[experts] (LDS), sc[E] unmasked tokens, sc[E + 1] choices out of range
 template <typename T, int L, int NI, int NT>
 __device__ __forceinline__ void count_tile(const BArgs& a, int64_t t0, int64_t t1, unsigned* sc) {
@@ -258,17 +279,20 @@ __device__ __forceinline__ void count_tile(const BArgs& a, int64_t t0, int64_t t
     return;
   }
   int cnt[G::PL] = {};
-  typename Key<T>::U guess = Key<T>::of((T)1.0f);
   int64_t t = t0 + wave * G::TW;
   if (t >= t1) return;
   Scores<T, L, NI> s, next;
   s.load(a, t + lane / L, t1);
+  next.load(a, t + STEP + lane / L, t1);
+  typename Key<T>::U guess = first_guess<T, L, NI>(s.x, a.z);
 #pragma clang loop unroll(disable)
-  for (; t < t1; t += STEP, s = next) {
-    next.load(a, t + STEP + lane / L, t1);  // on its way while this one is looked through
+  for (;;) {
     const bool on = s.on && t + lane / L < t1;
     live += on;
     choose<T, L, NI>(s.x, on, a.k, guess, cnt);
+    t += STEP, s = next;
+    if (t >= t1) break;
+    next.load(a, t + STEP + lane / L, t1);  // on its way while this one is looked through
   }
 #pragma unroll
   for (int i = 0; i < NI; ++i)
@@ -514,6 +538,10 @@ extern "C" pg_status pg_balance_value_and_gradient(pg_ctx* c, const pg_balance* 
     a.groups = b->groups, a.ntiles = b->ntiles, a.tokens = b->tokens, a.tile_tokens = b->tile_tokens, a.E = b->experts, a.k = b->k, a.cbits = b->chosen_bits;
     a.copies = (unsigned)b->copies;
     a.lam_e_k = b->lam * b->experts / b->k;
+    // (the normal distribution's quantile by the rational approximation 26.2.23 of Abramowitz and Stegun, good to 5e-4)
+    const double share = (double)b->k / b->experts, q = std::sqrt(-2.0 * std::log(std::max(std::min(share, 1.0 - share), 1e-4)));
+    const double tail = q - (2.515517 + q * (0.802853 + q * 0.010328)) / (1.0 + q * (1.432788 + q * (0.189269 + q * 0.001308)));
+    a.z = (float)(share <= 0.5 ? tail : -tail);
     a.partials = c->red_partials, a.out = out, a.counter = c->row_tickets, a.value = value;
     const bool whole = b->whole != 0;
     if (dtype == PG_F32) PG_TRY(run<float>(c, a, whole));
