@@ -589,8 +589,10 @@ struct RowsGeom {
 };
 
 template <typename T, int NT, int NV, bool tail, bool two>
-__global__ __launch_bounds__((NT < 256 ? 256 : NT), sizeof(T) == 8 ? 2 : 4) void distill_rows(DArgs) {
-  // (Float64 in 128 registers spills some eighty of them: two waves to a SIMD, and no workgroup of 1024 threads)
+__global__ __launch_bounds__((NT < 256 ? 256 : NT), sizeof(T) == 8 ? 2 : (NT == 64 && NV <= 2 && !tail && !two ? 8 : 4)) void distill_rows(DArgs) {
+  // (Waves to a SIMD.  Float64 in 128 registers spills some eighty of them: two, and no workgroup of 1024 threads.  Short rows wait for
+  // their lists and each other's lines rather than for bandwidth: eight, 65536 x 500 f16 91 us, 104 with the six that 80 registers
+  // allow; the other modes spill then and are no faster, 65536 x 500 f32 with an outside class 94 against 91.)
 
   // The arguments stay in memory and are read where they are used: hoisted out of the row loop they fill the scalar registers and
   // spill into vector ones
